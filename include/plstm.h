@@ -279,6 +279,93 @@ PLSTM_API int32_t plstm_hidden_update(const void* gate_proj, int32_t batch, int3
                             void* h_state, float* c_state, void* out, void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* ---- training and streaming operators ---------------------------------------
+ * What a trainable stack of recurrent layers needs around and instead of the
+ * LSTM (no counterpart in the reference): the gated scan, layer norm, dropout
+ * and the residual step that fuses the last two.  Every call only enqueues work
+ * on `stream`, allocates nothing and is safe under stream capture.  Sizes are
+ * element counts, strides are in elements, and the last axis of every tensor is
+ * contiguous.  No pointer alignment beyond the element's own is required
+ * (16-byte aligned rows take the vector kernels). */
+
+/* Gated scan: the recurrence of an LSTM layer whose gates do not look back,
+ *   c_t = sigmoid(f_t) c_{t-1} + sigmoid(i_t) tanh(g_t),  h_t = sigmoid(o_t) tanh(c_t),
+ * over gate projections [batch][seq_len][4 * hidden] in the gate order i, f, g, o
+ * (plstm_hidden_update with W_hh = 0).  lengths (int32 [batch], device, or NULL =
+ * seq_len; values are clamped to [0, seq_len]): from a row's length on the state
+ * stands still, h is zero and the gates are not read.  The state is f32. */
+typedef struct plstm_scan_desc {
+  int32_t batch, seq_len, hidden;
+  int32_t dtype;                                   /* PLSTM_F32 / _F16 / _BF16: gates, h and their gradients */
+  int32_t device;                                  /* CUDA device ordinal the pointers live on */
+  int32_t reserved;                                /* 0 */
+  int64_t gates_batch_stride, gates_time_stride;   /* gates */
+  int64_t h_batch_stride, h_time_stride;           /* h (forward), dh (backward; strides of 0 broadcast it) */
+  int64_t dgates_batch_stride, dgates_time_stride; /* dgates (backward) */
+} plstm_scan_desc;
+/* Bytes of the states the forward keeps for the backward (one f32 state for every
+ * PLSTM_SCAN_SEGMENT steps). */
+#define PLSTM_SCAN_SEGMENT 8
+PLSTM_API int32_t plstm_gated_scan_checkpoint_size(const plstm_scan_desc* d, size_t* bytes);
+/* c0 [batch][hidden] f32 (NULL = zeros); c_n [batch][hidden] f32, may be c0 itself
+ * (streaming); checkpoints: plstm_gated_scan_checkpoint_size bytes, or NULL when no
+ * backward follows. */
+PLSTM_API int32_t plstm_gated_scan_forward(const plstm_scan_desc* d, const void* gates, const int32_t* lengths,
+                                           const float* c0, void* h, float* c_n, float* checkpoints, void* stream);
+/* dh (NULL = zeros) and dc_n (f32, NULL = zeros) are the gradients of h and c_n;
+ * dgates receives the gradient of the gates (zero past each length), dc0 (f32, NULL =
+ * not wanted) that of c0. */
+PLSTM_API int32_t plstm_gated_scan_backward(const plstm_scan_desc* d, const void* gates, const int32_t* lengths,
+                                            const float* checkpoints, const void* dh, const float* dc_n, void* dgates,
+                                            float* dc0, void* stream);
+
+/* Dropout.  Element e of the row-major flattened tensor is kept where word e % 4 of
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) at counter words (e / 4 low, e / 4
+ * high, offset low, offset high) under key (seed low, seed high) is >= floor(p * 2^32);
+ * kept elements are scaled by 1 / (1 - p), dropped ones are zero whatever they hold.
+ * The mask is never stored: a backward calls again with the same seed and offset. */
+typedef struct plstm_dropout_desc {
+  double p;                  /* probability of dropping, in [0, 1] */
+  uint64_t seed, offset;
+  const uint64_t* seed_ptr;  /* device: read instead of `seed` when not NULL (graph replays with new masks) */
+} plstm_dropout_desc;
+/* y = dropout(x), or residual + dropout(x).  x is x_dtype, residual and y are y_dtype. */
+PLSTM_API int32_t plstm_dropout(const plstm_dropout_desc* drop, int64_t n, const void* x, int32_t x_dtype,
+                                const void* residual, void* y, int32_t y_dtype, int32_t device, void* stream);
+
+/* Layer norm over the last axis, y = (v - mean) / sqrt(var + eps) * weight + bias, of
+ * v = x, or, with a residual, of v = z = residual + dropout(x) as stored in z's type. */
+typedef struct plstm_norm_desc {
+  int64_t rows;
+  int32_t cols;              /* 1 .. PLSTM_NORM_MAX_COLS */
+  int32_t x_dtype;           /* x, y, dy, dx */
+  int32_t z_dtype;           /* residual, z, dz, dresidual: x_dtype or PLSTM_F32 */
+  int32_t w_dtype;           /* weight, bias and their gradients: x_dtype or PLSTM_F32 */
+  int32_t device;
+  float eps;
+  int64_t x_stride;          /* row strides; z, y and the gradients of x and residual are contiguous */
+  int64_t residual_stride;
+  int64_t dy_stride;
+  int64_t dz_stride;
+} plstm_norm_desc;
+#define PLSTM_NORM_MAX_COLS 16384
+/* weight and bias may be NULL (1 and 0).  residual NULL: plain layer norm, z is not
+ * written and drop must be NULL.  drop NULL: no dropout.  stats (f32 [2][rows]: mean,
+ * then 1 / sqrt(var + eps)) is what the backward needs, or NULL. */
+PLSTM_API int32_t plstm_layer_norm_forward(const plstm_norm_desc* d, const plstm_dropout_desc* drop, const void* x,
+                                           const void* residual, const void* weight, const void* bias, void* z,
+                                           void* y, float* stats, void* stream);
+PLSTM_API int32_t plstm_layer_norm_backward_workspace_size(const plstm_norm_desc* d, size_t* bytes);
+/* v: the forward's normalised tensor (x with row stride x_stride, or z with row stride
+ * cols when `fused` is not 0).  dy, dz: gradients of y and z (dz may be NULL).  dresidual
+ * (z_dtype) receives dz plus the norm's gradient, dx (x_dtype) that gradient through the
+ * dropout; without `fused` dresidual must be NULL and dx is the norm's gradient.
+ * dweight / dbias (w_dtype) may be NULL. */
+PLSTM_API int32_t plstm_layer_norm_backward(const plstm_norm_desc* d, const plstm_dropout_desc* drop, int32_t fused,
+                                            const void* dy, const void* dz, const void* v, const void* weight,
+                                            const float* stats, void* dx, void* dresidual, void* dweight,
+                                            void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- instrumentation (no counterpart in the reference beyond its
  * MIOPEN_ADAPTIVE_LSTM_PROFILE per-layer CUDA-event timings,
  * miopen_adaptive_lstm_hip/model.py:685-690, 1025-1052) ----------------------- */

@@ -19,6 +19,8 @@ from . import adaptive, adaptive_ext, ext
 from ._lib import PlstmError, PlstmUnavailable
 from .api import convert_lstm_module, convert_model_copy, convert_regressor_module, replace_lstm_inplace
 from .core import PackedWeights, check_device_status, lstm_linear_forward, select_backend, unique_rows
+from .gated import GatedScanLayer, GatedScanRegressor
+from .ops import dropout, dropout_add_layer_norm, gated_scan, gated_scan_step, layer_norm
 from .model import (NativeModuleFallback, PersistentLSTM, PersistentLSTM4LayerRegressor, PersistentLSTMRegressor,
                     StandardLSTMRegressor)
 
@@ -37,6 +39,13 @@ __all__ = [
     "select_backend",
     "unique_rows",
     "check_device_status",
+    "gated_scan",
+    "gated_scan_step",
+    "layer_norm",
+    "dropout",
+    "dropout_add_layer_norm",
+    "GatedScanLayer",
+    "GatedScanRegressor",
     "PlstmError",
     "PlstmUnavailable",
     "ext",

@@ -44,7 +44,33 @@ class Desc(ctypes.Structure):
         "w_layout", "flags", "backend", "timeout_ms", "device")]
 
 
+class ScanDesc(ctypes.Structure):
+    """plstm_scan_desc."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "seq_len", "hidden", "dtype", "device", "reserved")] + \
+        [(n, ctypes.c_int64) for n in ("gates_batch_stride", "gates_time_stride", "h_batch_stride", "h_time_stride",
+                                       "dgates_batch_stride", "dgates_time_stride")]
+
+
+class DropoutDesc(ctypes.Structure):
+    """plstm_dropout_desc."""
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                ("seed_ptr", ctypes.c_void_p)]
+
+
+class NormDesc(ctypes.Structure):
+    """plstm_norm_desc."""
+    _fields_ = [("rows", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("cols", "x_dtype", "z_dtype", "w_dtype", "device")] + \
+        [("eps", ctypes.c_float)] + \
+        [(n, ctypes.c_int64) for n in ("x_stride", "residual_stride", "dy_stride", "dz_stride")]
+
+
+NORM_MAX_COLS = 16384
+
 _DP = ctypes.POINTER(Desc)
+_SDP = ctypes.POINTER(ScanDesc)
+_RDP = ctypes.POINTER(DropoutDesc)
+_NDP = ctypes.POINTER(NormDesc)
 PROTOTYPES = {
     "plstm_abi_version": (_I32, []),
     "plstm_last_error": (ctypes.c_char_p, []),
@@ -69,6 +95,13 @@ PROTOTYPES = {
     "plstm_input_gemm": (_I32, [_P, _I32, _I32, _P, _I32, _I32, _P, _P]),
     "plstm_hidden_update_workspace_size": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_SZ)]),
     "plstm_hidden_update": (_I32, [_P, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P, _P, _SZ, _P]),
+    "plstm_gated_scan_checkpoint_size": (_I32, [_SDP, ctypes.POINTER(_SZ)]),
+    "plstm_gated_scan_forward": (_I32, [_SDP, _P, _P, _P, _P, _P, _P, _P]),
+    "plstm_gated_scan_backward": (_I32, [_SDP, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "plstm_dropout": (_I32, [_RDP, ctypes.c_int64, _P, _I32, _P, _P, _I32, _I32, _P]),
+    "plstm_layer_norm_forward": (_I32, [_NDP, _RDP, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "plstm_layer_norm_backward_workspace_size": (_I32, [_NDP, ctypes.POINTER(_SZ)]),
+    "plstm_layer_norm_backward": (_I32, [_NDP, _RDP, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "plstm_diag_tmem_layout": (_I32, [_P, _P]),
     "plstm_diag_step_latency": (_I32, [_I32, _I32, _I32, _P, _I32, _P]),
     "plstm_launch_count": (ctypes.c_int64, []),

@@ -21,8 +21,8 @@ LIB = os.path.join(LIB_DIR, "libplstm.so")
 OBJ_DIR_BC = os.path.join(HERE, "lib", "obj_bc")
 LIB_BC = os.path.join(LIB_DIR, "libplstm_bc.so")
 SOURCES = ["plstm_abi.cu", "plstm_simt.cu", "plstm_tc.cu", "plstm_tcl.cu", "plstm_gemm.cu", "plstm_misc.cu",
-           "plstm_noalloc.cu", "plstm_dedupe.cu"]
-HEADERS = ["plstm_common.cuh", "sm100_ptx.cuh"]
+           "plstm_noalloc.cu", "plstm_dedupe.cu", "plstm_scan.cu", "plstm_norm.cu", "plstm_dropout.cu"]
+HEADERS = ["plstm_common.cuh", "plstm_ops.cuh", "sm100_ptx.cuh"]
 NVCC = os.environ.get("NVCC", "nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",

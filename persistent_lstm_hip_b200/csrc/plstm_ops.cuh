@@ -1,0 +1,113 @@
+// plstm_ops.cuh — shared device code of the training and streaming operators
+// (plstm_scan.cu, plstm_norm.cu, plstm_dropout.cu).
+#pragma once
+
+#include "plstm_common.cuh"
+
+namespace plstm {
+namespace ops {
+
+constexpr int kSMs = 148;  // B200
+
+// V consecutive elements, loaded and stored with one instruction (V * sizeof(T) <= 16).
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& v) {
+  *reinterpret_cast<Vec<T, V>*>(p) = v;
+}
+
+inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+inline bool dtype_ok(int32_t dt) { return dt == PLSTM_F32 || dt == PLSTM_F16 || dt == PLSTM_BF16; }
+
+// ---- Philox4x32-10 ------------------------------------------------------------------------
+// Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3" (SC 2011): ten
+// rounds of two 32 x 32 -> 64-bit products and key additions (Weyl sequence) on a 128-bit
+// counter.  One call gives the words of four consecutive elements.
+__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint64_t seed) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// A dropout call as the kernels take it.
+struct Drop {
+  uint64_t seed, offset;
+  const uint64_t* seed_ptr;
+  uint32_t threshold;  // keep where word >= threshold
+  float scale;
+  int mode;            // 0: keep everything, 1: draw, 2: drop everything (p = 1)
+};
+
+__device__ __forceinline__ uint64_t drop_seed(const Drop& d) { return d.seed_ptr != nullptr ? *d.seed_ptr : d.seed; }
+
+// x / (1 - p) where the word keeps the element, else 0 (whatever x is).  The explicit
+// rounding keeps the compiler from contracting the product with a later sum, so that the
+// fused and the separate calls give the same bits.
+__device__ __forceinline__ float drop_one(const Drop& d, uint32_t word, float x) {
+  return word >= d.threshold ? __fmul_rn(x, d.scale) : 0.0f;
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& w, int k) {
+  return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+}
+
+// Applies the dropout to the V elements from flattened index e on.  V = 4 or 8 needs e % 4 == 0.
+template <int V>
+__device__ __forceinline__ void drop_vec(const Drop& d, uint64_t seed, int64_t e, float (&x)[V]) {
+  if (d.mode == 0) return;
+  if (d.mode == 2) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[k] = 0.0f;
+    return;
+  }
+  if constexpr (V == 1) {
+    x[0] = drop_one(d, word_of(philox((uint64_t)e >> 2, d.offset, seed), (int)(e & 3)), x[0]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const uint4 w = philox(((uint64_t)e >> 2) + q, d.offset, seed);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[4 * q + k] = drop_one(d, word_of(w, k), x[4 * q + k]);
+    }
+  }
+}
+
+// Checks a descriptor and fills the kernel's form of it (NULL: no dropout).
+inline int32_t make_drop(const plstm_dropout_desc* d, Drop* out) {
+  *out = Drop{0, 0, nullptr, 0, 1.0f, 0};
+  if (d == nullptr) return PLSTM_OK;
+  PLSTM_CHECK_ARG(d->p >= 0.0 && d->p <= 1.0, "dropout: p must be in [0, 1]");
+  out->seed = d->seed;
+  out->offset = d->offset;
+  out->seed_ptr = d->seed_ptr;
+  PLSTM_CHECK_ARG(aligned_to(d->seed_ptr, 8), "dropout: seed_ptr must be 8-byte aligned");
+  if (d->p == 0.0) return PLSTM_OK;
+  if (d->p == 1.0) {
+    out->mode = 2;
+    return PLSTM_OK;
+  }
+  out->mode = 1;
+  out->threshold = (uint32_t)(d->p * 4294967296.0);
+  out->scale = (float)(1.0 / (1.0 - d->p));
+  return PLSTM_OK;
+}
+
+}  // namespace ops
+}  // namespace plstm

@@ -30,14 +30,14 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(Drop d, int64_t n, co
       for (int k = 0; k < E; k += VX) {
         const Vec<TX, VX> in = load_vec<TX, VX>(x + e + k);
 #pragma unroll
-        for (int j = 0; j < VX; ++j) v[k + j] = to_f32(in.v[j]);
+        for (int j = 0; j < VX; ++j) v[k + j] = in.get(j);
       }
       if (residual != nullptr) {
 #pragma unroll
         for (int k = 0; k < E; k += VY) {
           const Vec<TY, VY> in = load_vec<TY, VY>(residual + e + k);
 #pragma unroll
-          for (int j = 0; j < VY; ++j) r[k + j] = to_f32(in.v[j]);
+          for (int j = 0; j < VY; ++j) r[k + j] = in.get(j);
         }
       }
     } else {
@@ -57,9 +57,11 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(Drop d, int64_t n, co
       constexpr int VY = 16 / sizeof(TY) < E ? 16 / sizeof(TY) : E;
 #pragma unroll
       for (int k = 0; k < E; k += VY) {
-        Vec<TY, VY> out;
+        float part[VY];
 #pragma unroll
-        for (int j = 0; j < VY; ++j) out.v[j] = from_f32<TY>(v[k + j]);
+        for (int j = 0; j < VY; ++j) part[j] = v[k + j];
+        Vec<TY, VY> out;
+        out.set(part);
         store_vec<TY, VY>(y + e + k, out);
       }
     } else {

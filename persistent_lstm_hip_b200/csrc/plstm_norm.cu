@@ -62,11 +62,25 @@ __device__ __forceinline__ void row_sum(float (&a)[NV], int tpr, float* scratch)
   }
 }
 
-// V elements of a weight in its own type (NULL: `none`).
-template <int V>
+// V elements of a weight that has x's type or f32 (NULL: `none`).  V > 1 needs 16-byte aligned weights.
+template <typename TX, int V>
 __device__ __forceinline__ void load_weight(const void* w, int dtype, int col, float none, float (&out)[V]) {
+  if (w == nullptr) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) out[k] = w != nullptr ? load_any(w, dtype, col + k) : none;
+    for (int k = 0; k < V; ++k) out[k] = none;
+  } else if (sizeof(TX) == 4 || dtype == PLSTM_F32) {
+    constexpr int VW = V < 4 ? V : 4;
+#pragma unroll
+    for (int q = 0; q < V; q += VW) {
+      const Vec<float, VW> in = load_vec<float, VW>(static_cast<const float*>(w) + col + q);
+#pragma unroll
+      for (int k = 0; k < VW; ++k) out[q + k] = in.get(k);
+    }
+  } else {
+    const Vec<TX, V> in = load_vec<TX, V>(static_cast<const TX*>(w) + col);
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = in.get(k);
+  }
 }
 
 template <typename TX, typename TZ, int V, int CH, bool FUSED>
@@ -88,7 +102,7 @@ __global__ void __launch_bounds__(max_threads(V)) norm_forward_kernel(NormArgs a
       if (live && col < a.cols) {
         const Vec<TX, V> in = load_vec<TX, V>(static_cast<const TX*>(a.x) + row * a.x_stride + col);
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[c][k] = to_f32(in.v[k]);
+        for (int k = 0; k < V; ++k) v[c][k] = in.get(k);
         if constexpr (FUSED) {
           const int64_t e = row * a.cols + col;
           drop_vec<V>(a.drop, seed, e, v[c]);
@@ -97,12 +111,13 @@ __global__ void __launch_bounds__(max_threads(V)) norm_forward_kernel(NormArgs a
 #pragma unroll
           for (int q = 0; q < V; q += VZ) {
             const Vec<TZ, VZ> r = load_vec<TZ, VZ>(res + q);
-            Vec<TZ, VZ> z;
+            float part[VZ];
 #pragma unroll
-            for (int k = 0; k < VZ; ++k) {
-              z.v[k] = from_f32<TZ>(__fadd_rn(to_f32(r.v[k]), v[c][q + k]));
-              v[c][q + k] = to_f32(z.v[k]);  // the norm is of z as stored
-            }
+            for (int k = 0; k < VZ; ++k) part[k] = __fadd_rn(r.get(k), v[c][q + k]);
+            Vec<TZ, VZ> z;
+            z.set(part);
+#pragma unroll
+            for (int k = 0; k < VZ; ++k) v[c][q + k] = z.get(k);  // the norm is of z as stored
             store_vec<TZ, VZ>(static_cast<TZ*>(a.z) + e + q, z);
           }
         }
@@ -138,11 +153,12 @@ __global__ void __launch_bounds__(max_threads(V)) norm_forward_kernel(NormArgs a
       const int col = (c * tpr + lane) * V;
       if (col < a.cols) {
         float w[V], b[V];
-        load_weight<V>(a.weight, a.w_dtype, col, 1.0f, w);
-        load_weight<V>(a.bias, a.w_dtype, col, 0.0f, b);
-        Vec<TX, V> out;
+        load_weight<TX, V>(a.weight, a.w_dtype, col, 1.0f, w);
+        load_weight<TX, V>(a.bias, a.w_dtype, col, 0.0f, b);
 #pragma unroll
-        for (int k = 0; k < V; ++k) out.v[k] = from_f32<TX>(v[c][k] * rstd * w[k] + b[k]);
+        for (int k = 0; k < V; ++k) w[k] = v[c][k] * rstd * w[k] + b[k];
+        Vec<TX, V> out;
+        out.set(w);
         store_vec<TX, V>(static_cast<TX*>(a.y) + row * a.cols + col, out);
       }
     }
@@ -181,13 +197,13 @@ __global__ void __launch_bounds__(max_threads(V)) norm_backward_kernel(NormArgs 
         for (int q = 0; q < V; q += VV) {
           const Vec<TV, VV> in = load_vec<TV, VV>(static_cast<const TV*>(a.v) + row * v_stride + col + q);
 #pragma unroll
-          for (int k = 0; k < VV; ++k) xh[c][q + k] = (to_f32(in.v[k]) - mean) * rstd;
+          for (int k = 0; k < VV; ++k) xh[c][q + k] = (in.get(k) - mean) * rstd;
         }
         float w[V];
-        load_weight<V>(a.weight, a.w_dtype, col, 1.0f, w);
+        load_weight<TX, V>(a.weight, a.w_dtype, col, 1.0f, w);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float d = to_f32(dy.v[k]);
+          const float d = dy.get(k);
           dw[c][k] += d * xh[c][k];
           db[c][k] += d;
           g[c][k] = d * w[k];
@@ -213,15 +229,17 @@ __global__ void __launch_bounds__(max_threads(V)) norm_backward_kernel(NormArgs 
             for (int q = 0; q < V; q += VV) {
               const Vec<TV, VV> dz = load_vec<TV, VV>(static_cast<const TV*>(a.dz) + row * a.dz_stride + col + q);
 #pragma unroll
-              for (int k = 0; k < VV; ++k) dv[q + k] += to_f32(dz.v[k]);
+              for (int k = 0; k < VV; ++k) dv[q + k] += dz.get(k);
             }
           }
           if (a.dres != nullptr) {
 #pragma unroll
             for (int q = 0; q < V; q += VV) {
-              Vec<TV, VV> out;
+              float part[VV];
 #pragma unroll
-              for (int k = 0; k < VV; ++k) out.v[k] = from_f32<TV>(dv[q + k]);
+              for (int k = 0; k < VV; ++k) part[k] = dv[q + k];
+              Vec<TV, VV> out;
+              out.set(part);
               store_vec<TV, VV>(static_cast<TV*>(a.dres) + e + q, out);
             }
           }
@@ -230,8 +248,7 @@ __global__ void __launch_bounds__(max_threads(V)) norm_backward_kernel(NormArgs 
         }
         if (a.dx != nullptr) {
           Vec<TX, V> out;
-#pragma unroll
-          for (int k = 0; k < V; ++k) out.v[k] = from_f32<TX>(dv[k]);
+          out.set(dv);
           store_vec<TX, V>(static_cast<TX*>(a.dx) + e, out);
         }
       }
@@ -422,7 +439,8 @@ int32_t plstm_layer_norm_forward(const plstm_norm_desc* d, const plstm_dropout_d
   DeviceGuard guard;
   if (const int32_t rc = guard.enter(d->device)) return rc;
   const bool vec = d->cols % (16 / xs) == 0 && rows16(x, d->x_stride, d->x_dtype) && aligned16(y) &&
-                   rows16(residual, d->residual_stride, d->z_dtype) && aligned16(z);
+                   rows16(residual, d->residual_stride, d->z_dtype) && aligned16(z) && aligned16(weight) &&
+                   aligned16(bias);
   const Split s = make_split(*d, vec);
   a.rows = d->rows;
   a.cols = d->cols;
@@ -493,7 +511,7 @@ int32_t plstm_layer_norm_backward(const plstm_norm_desc* d, const plstm_dropout_
   if (d->rows > 0 && (grads || dx != nullptr || dresidual != nullptr)) {
     const bool vec = d->cols % (16 / xs) == 0 && rows16(dy, d->dy_stride, d->x_dtype) &&
                      rows16(v, fused ? d->cols : d->x_stride, d->z_dtype) && rows16(dz, d->dz_stride, d->z_dtype) &&
-                     aligned16(dx) && aligned16(dresidual);
+                     aligned16(dx) && aligned16(dresidual) && aligned16(weight);
     const Split s = make_split(*d, vec);
     parts = (int)row_ctas(*d, s, backward_per_sm(s));
     a.rows = d->rows;

@@ -2,6 +2,8 @@
 // (plstm_scan.cu, plstm_norm.cu, plstm_dropout.cu).
 #pragma once
 
+#include <type_traits>
+
 #include "plstm_common.cuh"
 
 namespace plstm {
@@ -9,19 +11,79 @@ namespace ops {
 
 constexpr int kSMs = 148;  // B200
 
-// V consecutive elements, loaded and stored with one instruction (V * sizeof(T) <= 16).
+// N bytes moved by one load or store.
+template <int N>
+struct Word;
+template <>
+struct Word<2> {
+  using type = unsigned short;
+};
+template <>
+struct Word<4> {
+  using type = uint32_t;
+};
+template <>
+struct Word<8> {
+  using type = uint2;
+};
+template <>
+struct Word<16> {
+  using type = uint4;
+};
+
+// V consecutive elements as they lie in memory, moved by one instruction (V * sizeof(T) <= 16).
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Vec {
-  T v[V];
+struct Vec {
+  union {
+    typename Word<V * sizeof(T)>::type word;
+    uint32_t w[V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1];
+  };
+  __device__ __forceinline__ float get(int k) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[k]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      // bf16 is the upper half of an f32.
+      if constexpr (V == 1) return __uint_as_float((uint32_t)word << 16);
+      return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    } else {
+      if constexpr (V == 1) return __half2float(__ushort_as_half(word));
+      return __half2float(__ushort_as_half((unsigned short)(k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu)));
+    }
+  }
+  // Rounds all V values to nearest even.
+  __device__ __forceinline__ void set(const float (&f)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) w[k] = __float_as_uint(f[k]);
+    } else if constexpr (V == 1) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        word = __bfloat16_as_ushort(__float2bfloat16_rn(f[0]));
+      else
+        word = __half_as_ushort(__float2half_rn(f[0]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; k += 2) {
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(f[k], f[k + 1]);
+          w[k >> 1] = *reinterpret_cast<const uint32_t*>(&p);
+        } else {
+          const __half2 p = __floats2half2_rn(f[k], f[k + 1]);
+          w[k >> 1] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+      }
+    }
+  }
 };
 
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
-  return *reinterpret_cast<const Vec<T, V>*>(p);
+  Vec<T, V> v;
+  v.word = *reinterpret_cast<const typename Word<V * sizeof(T)>::type*>(p);
+  return v;
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& v) {
-  *reinterpret_cast<Vec<T, V>*>(p) = v;
+  *reinterpret_cast<typename Word<V * sizeof(T)>::type*>(p) = v.word;
 }
 
 inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }

@@ -50,28 +50,201 @@ struct ScanArgs {
   float* dc0;
 };
 
-// f32 inputs use CUDA's accurate functions; for 16-bit inputs the exponential's and the
-// division's fast forms (a few units in 2^-23 for the arguments gates take) are far below the
-// inputs' own 2^-9 or 2^-12, and tanh takes its odd series below 0.3, where 1 - 2 / (1 + e^2x)
-// would cancel.
-template <typename T>
-__device__ __forceinline__ float sigmoid_of(float x) {
-  if constexpr (sizeof(T) == 4) return sigmoid_acc(x);
-  return __fdividef(1.0f, 1.0f + __expf(-x));
+// ---- packed arithmetic -------------------------------------------------------------------------
+// V f32 values of neighbouring channels.  Two of them go through the f32x2 instructions, which do
+// two operations for one issue slot; the special-function unit takes them one by one.
+template <int V>
+struct F;
+template <>
+struct F<1> {
+  float x;
+  __device__ __forceinline__ float get(int) const { return x; }
+  static __device__ __forceinline__ F of(float a) { return {a}; }
+  static __device__ __forceinline__ F of(const float (&a)[1]) { return {a[0]}; }
+};
+template <>
+struct F<2> {
+  uint64_t p;
+  __device__ __forceinline__ float get(int k) const { return __uint_as_float((uint32_t)(k ? p >> 32 : p)); }
+  static __device__ __forceinline__ F of(float lo, float hi) {
+    return {(uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo)};
+  }
+  static __device__ __forceinline__ F of(float a) { return of(a, a); }
+  static __device__ __forceinline__ F of(const float (&a)[2]) { return of(a[0], a[1]); }
+};
+__device__ __forceinline__ F<1> fma(F<1> a, F<1> b, F<1> c) { return {fmaf(a.x, b.x, c.x)}; }
+__device__ __forceinline__ F<1> operator*(F<1> a, F<1> b) { return {a.x * b.x}; }
+__device__ __forceinline__ F<1> operator+(F<1> a, F<1> b) { return {a.x + b.x}; }
+__device__ __forceinline__ F<2> fma(F<2> a, F<2> b, F<2> c) {
+  F<2> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.p) : "l"(a.p), "l"(b.p), "l"(c.p));
+  return r;
 }
-template <typename T>
-__device__ __forceinline__ float tanh_of(float x) {
-  if constexpr (sizeof(T) == 4) return tanh_acc(x);
-  const float s = x * x;
-  const float small = x * (1.0f + s * (-1.0f / 3 + s * (2.0f / 15 + s * (-17.0f / 315 + s * (62.0f / 2835)))));
-  const float large = 1.0f - __fdividef(2.0f, 1.0f + __expf(2.0f * x));
-  return fabsf(x) < 0.3f ? small : large;
+__device__ __forceinline__ F<2> operator*(F<2> a, F<2> b) {
+  F<2> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
+  return r;
+}
+__device__ __forceinline__ F<2> operator+(F<2> a, F<2> b) {
+  F<2> r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
+  return r;
+}
+template <int V, typename Fn>
+__device__ __forceinline__ F<V> each(F<V> a, Fn fn) {
+  float r[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) r[k] = fn(a.get(k));
+  return F<V>::of(r);
+}
+// a * b + 1 and the like with a constant in every lane.
+template <int V>
+__device__ __forceinline__ F<V> fma(F<V> a, F<V> b, float c) { return fma(a, b, F<V>::of(c)); }
+template <int V>
+__device__ __forceinline__ F<V> one_plus(F<V> a) { return a + F<V>::of(1.0f); }
+template <int V>
+__device__ __forceinline__ F<V> one_minus(F<V> a) { return fma(a, F<V>::of(-1.0f), F<V>::of(1.0f)); }
+
+// One special-function instruction each; results below 2^-126 come out as 0, 1 / inf as 0.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// max and min that keep a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// ---- gate functions ----------------------------------------------------------------------------
+// exp(s x) for s = -1 or -2.  exp = 2^(s log2(e) x) by the special-function unit is good to two
+// units in 2^-23 plus the rounding of the product, |x| units in 2^-24: far below 16-bit inputs' own
+// rounding.  For f32 (PRECISE) the product's rounding error is carried along: with t = fl(a x),
+// a = hi + lo, the error r = a x - t enters as 2^(t + r) = 2^t (1 + r ln 2).
+template <bool PRECISE, int V>
+__device__ __forceinline__ F<V> exp_of(F<V> x, float s) {
+  constexpr float kHi = 1.44269502162933349609375f;      // log2(e) to 24 bits
+  constexpr float kLo = 1.925963033500011079e-8f;        // log2(e) - kHi
+  constexpr float kLn2 = 0.693147180559945309f;
+  if constexpr (PRECISE) {
+    // Neither 2^t nor r overflows in here, and sigmoid(-87.6) is already below 2^-126.
+    x = each(x, [](float v) { return min_nan(max_nan(v, -87.6f), 87.6f); });
+    const F<V> t = x * F<V>::of(s * kHi);
+    const F<V> r = fma(x, F<V>::of(s * kLo), fma(x, F<V>::of(s * kHi), t * F<V>::of(-1.0f)));
+    const F<V> e = each(t, ex2);
+    return fma(e, r * F<V>::of(kLn2), e);
+  } else {
+    return each(x * F<V>::of(s * kHi), ex2);
+  }
+}
+template <bool PRECISE, int V>
+__device__ __forceinline__ F<V> sigmoid_f(F<V> x) {
+  return each(one_plus(exp_of<PRECISE>(x, -1.0f)), rcp);
+}
+// tanh(x) = num / den.  From 0.3 on (1 - e^-2x) / (1 + e^-2x), of x >= -9.1, where tanh rounds to
+// -1 and the exponential is still small enough to be multiplied with another; below 0.3, where
+// the difference would cancel, the odd series to x^9 (the next term is 4e-8 of the value).
+template <bool PRECISE, int V>
+__device__ __forceinline__ void tanh_parts(F<V> x, F<V>& num, F<V>& den) {
+  const F<V> e = exp_of<PRECISE>(each(x, [](float v) { return max_nan(v, -9.1f); }), -2.0f);
+  const F<V> s = x * x;
+  F<V> p = fma(s, F<V>::of(62.0f / 2835), -17.0f / 315);
+  p = fma(s, p, 2.0f / 15);
+  p = fma(s, p, -1.0f / 3);
+  p = fma(x * s, p, x);
+  const F<V> n = one_minus(e), d = one_plus(e);
+  float rn[V], rd[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const bool small = fabsf(x.get(k)) < 0.3f;
+    rn[k] = small ? p.get(k) : n.get(k);
+    rd[k] = small ? 1.0f : d.get(k);
+  }
+  num = F<V>::of(rn);
+  den = F<V>::of(rd);
+}
+template <bool PRECISE, int V>
+__device__ __forceinline__ F<V> tanh_f(F<V> x) {
+  F<V> num, den;
+  tanh_parts<PRECISE>(x, num, den);
+  return num * each(den, rcp);
+}
+// sigmoid(a) tanh(x) with one reciprocal.
+template <bool PRECISE, int V>
+__device__ __forceinline__ F<V> sigmoid_tanh(F<V> a, F<V> x) {
+  F<V> num, den;
+  tanh_parts<PRECISE>(x, num, den);
+  return num * each(one_plus(exp_of<PRECISE>(a, -1.0f)) * den, rcp);
 }
 
 template <int V>
-struct alignas(8 * V) Run {  // the action (A, b) of a run of steps on V channels
-  float a[V], b[V];
+struct alignas(8 * V) Run {  // the action c -> a c + b of a run of steps
+  F<V> a, b;
 };
+
+// Reads V elements; those past the length are given as the step that changes nothing.
+template <typename T>
+__device__ __forceinline__ uint32_t infinity_bits() {
+  return sizeof(T) == 4 ? 0x7f800000u : std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> constant_vec(uint32_t bits) {
+  Vec<T, V> v;
+  if constexpr (V * sizeof(T) == 2) {
+    v.word = (unsigned short)bits;
+  } else {
+#pragma unroll
+    for (int k = 0; k < (int)(V * sizeof(T) / 4); ++k) v.w[k] = bits;
+  }
+  return v;
+}
+template <typename T, int V>
+__device__ __forceinline__ F<V> widen(const Vec<T, V>& v) {
+  float r[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) r[k] = v.get(k);
+  return F<V>::of(r);
+}
+// Rounds to T; zero where the step is past the length.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(F<V> f, bool in) {
+  float r[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) r[k] = f.get(k);
+  Vec<T, V> v;
+  v.set(r);
+  if constexpr (V * sizeof(T) == 2) {
+    if (!in) v.word = 0;
+  } else {
+#pragma unroll
+    for (int k = 0; k < (int)(V * sizeof(T) / 4); ++k) v.w[k] = in ? v.w[k] : 0u;
+  }
+  return v;
+}
+template <int V>
+__device__ __forceinline__ F<V> load_state(const float* p, int64_t at, bool live) {
+  float r[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) r[k] = live && p != nullptr ? p[at + k] : 0.0f;
+  return F<V>::of(r);
+}
+template <int V>
+__device__ __forceinline__ void store_state(float* p, int64_t at, F<V> f) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) p[at + k] = f.get(k);
+}
 
 // Where a thread stands.
 template <int V>
@@ -92,71 +265,66 @@ struct Place {
   }
 };
 
-// The exchange between the threads that share a channel.  `own` is this thread's run; on return
-// `state` (the value entering the tile) has become the value entering this thread's run and
-// `carry` the value leaving the whole tile.  ORDER(s): the s-th segment or rank in running order.
+// The exchange between the threads that share a channel.  `own` is this thread's run; `carry`, the
+// state entering the tile, becomes the one leaving it.  Returns the state entering this thread's
+// run.  Runs are folded in running order (backward: from the last segment and rank to the first).
 template <int V, bool REVERSE>
 struct Exchange {
   Run<V>* segs;   // [2][seg][cl]
   Run<V>* ranks;  // [2][kMaxCluster][cl]
 
-  __device__ __forceinline__ void operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
-                                             float (&state)[V], float (&carry)[V]) const {
+  __device__ __forceinline__ F<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
+                                             F<V>& carry) const {
     const int parity = turn & 1;
     Run<V>* mine = segs + parity * p.seg * p.cl;
     const int order = REVERSE ? p.seg - 1 - at.seg : at.seg;
+    F<V> state = carry;
+    if (at.ranks == 1) {
+      if (p.seg == 1) {
+        carry = fma(own.a, carry, own.b);
+        return state;
+      }
+      mine[order * p.cl + at.cl] = own;
+      __syncthreads();
+      for (int s = 0; s < p.seg; ++s) {
+        if (s == order) state = carry;
+        const Run<V> r = mine[s * p.cl + at.cl];
+        carry = fma(r.a, carry, r.b);
+      }
+      return state;
+    }
     mine[order * p.cl + at.cl] = own;
     __syncthreads();
-    // The run of the CTA's segments before this thread's.
-    Run<V> pre;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      pre.a[k] = 1.0f;
-      pre.b[k] = 0.0f;
-    }
-    Run<V> all = pre;
+    // The run of the CTA's segments before this thread's, and of all of them.
+    Run<V> all{F<V>::of(1.0f), F<V>::of(0.0f)}, pre = all;
     for (int s = 0; s < p.seg; ++s) {
       if (s == order) pre = all;
       const Run<V> r = mine[s * p.cl + at.cl];
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        all.b[k] = r.a[k] * all.b[k] + r.b[k];
-        all.a[k] *= r.a[k];
-      }
+      all.b = fma(r.a, all.b, r.b);
+      all.a = r.a * all.a;
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) carry[k] = state[k];
-    if (at.ranks > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      Run<V>* slots = ranks + parity * kMaxCluster * p.cl;
-      const int rank_order = REVERSE ? at.ranks - 1 - at.rank : at.rank;
-      for (int r = at.seg; r < at.ranks; r += p.seg)  // the segments share the remote stores
-        cluster.map_shared_rank(slots, r)[rank_order * p.cl + at.cl] = all;
-      cluster.sync();
-      for (int r = 0; r < at.ranks; ++r) {
-        if (r == rank_order) {
-#pragma unroll
-          for (int k = 0; k < V; ++k) state[k] = carry[k];
-        }
-        const Run<V> q = slots[r * p.cl + at.cl];
-#pragma unroll
-        for (int k = 0; k < V; ++k) carry[k] = q.a[k] * carry[k] + q.b[k];
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) carry[k] = all.a[k] * carry[k] + all.b[k];
+    cg::cluster_group cluster = cg::this_cluster();
+    Run<V>* slots = ranks + parity * kMaxCluster * p.cl;
+    const int rank_order = REVERSE ? at.ranks - 1 - at.rank : at.rank;
+    for (int r = at.seg; r < at.ranks; r += p.seg)  // the segments share the remote stores
+      cluster.map_shared_rank(slots, r)[rank_order * p.cl + at.cl] = all;
+    cluster.sync();
+    for (int r = 0; r < at.ranks; ++r) {
+      if (r == rank_order) state = carry;
+      const Run<V> q = slots[r * p.cl + at.cl];
+      carry = fma(q.a, carry, q.b);
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) state[k] = pre.a[k] * state[k] + pre.b[k];
+    return fma(pre.a, state, pre.b);
   }
 };
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
-  extern __shared__ __align__(16) float smem[];
+  constexpr bool PRECISE = sizeof(T) == 4;
+  extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
-  Exchange<V, false> exchange{reinterpret_cast<Run<V>*>(smem),
-                              reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
+  const Exchange<V, false> exchange{reinterpret_cast<Run<V>*>(smem),
+                                    reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
   // Distributed shared memory may be written once every CTA of the cluster has started.
   if (cluster > 1) cg::this_cluster().sync();
   const int tile = kSeg * p.seg * cluster;
@@ -164,80 +332,56 @@ __global__ void __launch_bounds__(kMaxThreads) scan_forward_kernel(const __grid_
   const int segments = (p.T + kSeg - 1) / kSeg;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   T* h = static_cast<T*>(p.h) + at.b * p.h_sb + at.ch;
-  float carry[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k)
-    carry[k] = at.live && p.c0 != nullptr ? p.c0[(int64_t)at.b * p.H + at.ch + k] : 0.0f;
+  const int64_t state_at = (int64_t)at.b * p.H + at.ch;
+  F<V> carry = load_state<V>(p.c0, state_at, at.live);
   for (int turn = 0; turn < turns; ++turn) {
     const int t0 = turn * tile + (at.rank * p.seg + at.seg) * kSeg;
     Vec<T, V> raw[4][kSeg];
-#pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      if (at.live && t0 + j < at.len) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) raw[q][j] = load_vec<T, V>(gates + (t0 + j) * p.g_st + (int64_t)q * p.H);
-      }
-    }
-    float f[kSeg][V], u[kSeg][V];
-    Run<V> own;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      own.a[k] = 1.0f;
-      own.b[k] = 0.0f;
-    }
+    const T* from = gates + t0 * p.g_st;
 #pragma unroll
     for (int j = 0; j < kSeg; ++j) {
       const bool in = at.live && t0 + j < at.len;
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        f[j][k] = in ? sigmoid_of<T>(to_f32(raw[1][j].v[k])) : 1.0f;
-        u[j][k] = in ? sigmoid_of<T>(to_f32(raw[0][j].v[k])) * tanh_of<T>(to_f32(raw[2][j].v[k])) : 0.0f;
-        own.b[k] = f[j][k] * own.b[k] + u[j][k];
-        own.a[k] *= f[j][k];
+      for (int q = 0; q < 4; ++q) {
+        // f = 1, u = 0: an infinite forget gate over a zero candidate.
+        raw[q][j] = in ? load_vec<T, V>(from + (int64_t)q * p.H) : constant_vec<T, V>(q == 1 ? infinity_bits<T>() : 0);
       }
+      from += p.g_st;
     }
-    float c[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) c[k] = carry[k];
-    exchange(p, at, turn, own, c, carry);
-    if (at.live && p.ckpt != nullptr && t0 < at.len) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        p.ckpt[((int64_t)at.b * segments + t0 / kSeg) * p.H + at.ch + k] = c[k];
-    }
+    F<V> f[kSeg], u[kSeg];
+    Run<V> own{F<V>::of(1.0f), F<V>::of(0.0f)};
 #pragma unroll
     for (int j = 0; j < kSeg; ++j) {
-      if (at.live && t0 + j < p.T) {
-        Vec<T, V> out;
+      f[j] = sigmoid_f<PRECISE>(widen(raw[1][j]));
+      u[j] = sigmoid_tanh<PRECISE>(widen(raw[0][j]), widen(raw[2][j]));
+      own.b = fma(f[j], own.b, u[j]);
+      own.a = own.a * f[j];
+    }
+    F<V> c = exchange(p, at, turn, own, carry);
+    if (at.live && p.ckpt != nullptr && t0 < at.len)
+      store_state<V>(p.ckpt, ((int64_t)at.b * segments + t0 / kSeg) * p.H + at.ch, c);
+    T* to = h + t0 * p.h_st;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          c[k] = f[j][k] * c[k] + u[j][k];
-          const float o = t0 + j < at.len ? sigmoid_of<T>(to_f32(raw[3][j].v[k])) * tanh_of<T>(c[k]) : 0.0f;
-          out.v[k] = from_f32<T>(o);
-        }
-        store_vec<T, V>(h + (t0 + j) * p.h_st, out);
-      }
+    for (int j = 0; j < kSeg; ++j) {
+      c = fma(f[j], c, u[j]);
+      const Vec<T, V> out = narrow<T, V>(sigmoid_tanh<PRECISE>(widen(raw[3][j]), c), t0 + j < at.len);
+      if (at.live && t0 + j < p.T) store_vec<T, V>(to, out);
+      to += p.h_st;
     }
   }
   if (!at.live) return;
-  Vec<T, V> zero;
-#pragma unroll
-  for (int k = 0; k < V; ++k) zero.v[k] = from_f32<T>(0.0f);
   for (int64_t t = (int64_t)turns * tile + at.rank * p.seg + at.seg; t < p.T; t += p.seg * cluster)
-    store_vec<T, V>(h + t * p.h_st, zero);
-  if (at.rank == 0 && at.seg == 0) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) p.c_n[(int64_t)at.b * p.H + at.ch + k] = carry[k];
-  }
+    store_vec<T, V>(h + t * p.h_st, constant_vec<T, V>(0));
+  if (at.rank == 0 && at.seg == 0) store_state<V>(p.c_n, state_at, carry);
 }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
-  extern __shared__ __align__(16) float smem[];
+  constexpr bool PRECISE = sizeof(T) == 4;
+  extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
-  Exchange<V, true> exchange{reinterpret_cast<Run<V>*>(smem),
-                             reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
-  // Distributed shared memory may be written once every CTA of the cluster has started.
+  const Exchange<V, true> exchange{reinterpret_cast<Run<V>*>(smem),
+                                   reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
   if (cluster > 1) cg::this_cluster().sync();
   const int tile = kSeg * p.seg * cluster;
   const int turns = (at.len + tile - 1) / tile;
@@ -245,88 +389,60 @@ __global__ void __launch_bounds__(kMaxThreads) scan_backward_kernel(const __grid
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   const T* dh = p.dh != nullptr ? static_cast<const T*>(p.dh) + at.b * p.h_sb + at.ch : nullptr;
   T* dg = static_cast<T*>(p.dgates) + at.b * p.d_sb + at.ch;
-  Vec<T, V> zero;
-#pragma unroll
-  for (int k = 0; k < V; ++k) zero.v[k] = from_f32<T>(0.0f);
-  float carry[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k)
-    carry[k] = at.live && p.dc_n != nullptr ? p.dc_n[(int64_t)at.b * p.H + at.ch + k] : 0.0f;
+  const int64_t state_at = (int64_t)at.b * p.H + at.ch;
+  F<V> carry = load_state<V>(p.dc_n, state_at, at.live);
   for (int turn = 0; turn < turns; ++turn) {
     const int t0 = (turns - 1 - turn) * tile + (at.rank * p.seg + at.seg) * kSeg;
     Vec<T, V> raw[4][kSeg], rdh[kSeg];
-#pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      if (at.live && t0 + j < at.len) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) raw[q][j] = load_vec<T, V>(gates + (t0 + j) * p.g_st + (int64_t)q * p.H);
-        rdh[j] = dh != nullptr ? load_vec<T, V>(dh + (t0 + j) * p.h_st) : zero;
-      }
-    }
-    float c[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      c[k] = at.live && t0 < at.len ? p.ckpt[((int64_t)at.b * segments + t0 / kSeg) * p.H + at.ch + k] : 0.0f;
-    // Per step: f, e and what dc is multiplied with in the gradients of i, f and g.
-    float f[kSeg][V], e[kSeg][V], wi[kSeg][V], wf[kSeg][V], wg[kSeg][V];
+    const T* from = gates + t0 * p.g_st;
+    const T* dfrom = dh + t0 * p.h_st;
 #pragma unroll
     for (int j = 0; j < kSeg; ++j) {
       const bool in = at.live && t0 + j < at.len;
-      Vec<T, V> d_o = zero;
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        f[j][k] = 1.0f;
-        e[j][k] = 0.0f;
-        if (in) {
-          const float si = sigmoid_of<T>(to_f32(raw[0][j].v[k])), sf = sigmoid_of<T>(to_f32(raw[1][j].v[k]));
-          const float g = tanh_of<T>(to_f32(raw[2][j].v[k])), so = sigmoid_of<T>(to_f32(raw[3][j].v[k]));
-          const float d = to_f32(rdh[j].v[k]);
-          f[j][k] = sf;
-          wf[j][k] = c[k] * sf * (1.0f - sf);
-          wi[j][k] = g * si * (1.0f - si);
-          wg[j][k] = si * (1.0f - g * g);
-          c[k] = sf * c[k] + si * g;
-          const float tc = tanh_of<T>(c[k]);
-          e[j][k] = d * so * (1.0f - tc * tc);
-          d_o.v[k] = from_f32<T>(d * tc * so * (1.0f - so));
-        }
+      for (int q = 0; q < 4; ++q) {
+        raw[q][j] = in ? load_vec<T, V>(from + (int64_t)q * p.H) : constant_vec<T, V>(q == 1 ? infinity_bits<T>() : 0);
       }
-      if (at.live && t0 + j < p.T) store_vec<T, V>(dg + (t0 + j) * p.d_st + 3 * (int64_t)p.H, d_o);
+      rdh[j] = in && dh != nullptr ? load_vec<T, V>(dfrom) : constant_vec<T, V>(0);
+      from += p.g_st;
+      dfrom += p.h_st;
     }
-    Run<V> own;
+    F<V> c = load_state<V>(p.ckpt, ((int64_t)at.b * segments + t0 / kSeg) * p.H + at.ch, at.live && t0 < at.len);
+    // Per step: f, e and what dc is multiplied with in the gradients of i, f and g.
+    F<V> f[kSeg], e[kSeg], wi[kSeg], wf[kSeg], wg[kSeg];
+    T* to = dg + t0 * p.d_st;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      own.a[k] = 1.0f;
-      own.b[k] = 0.0f;
+    for (int j = 0; j < kSeg; ++j) {
+      const F<V> si = sigmoid_f<PRECISE>(widen(raw[0][j])), sf = sigmoid_f<PRECISE>(widen(raw[1][j]));
+      const F<V> g = tanh_f<PRECISE>(widen(raw[2][j])), so = sigmoid_f<PRECISE>(widen(raw[3][j]));
+      const F<V> d = widen(rdh[j]);
+      f[j] = sf;
+      wf[j] = c * (sf * one_minus(sf));
+      wi[j] = g * (si * one_minus(si));
+      wg[j] = si * one_minus(g * g);
+      c = fma(sf, c, si * g);
+      const F<V> tc = tanh_f<PRECISE>(c), dso = d * so;
+      e[j] = t0 + j < at.len ? dso * one_minus(tc * tc) : F<V>::of(0.0f);
+      const Vec<T, V> d_o = narrow<T, V>(dso * tc * one_minus(so), t0 + j < at.len);
+      if (at.live && t0 + j < p.T) store_vec<T, V>(to + 3 * (int64_t)p.H, d_o);
+      to += p.d_st;
     }
+    Run<V> own{F<V>::of(1.0f), F<V>::of(0.0f)};
 #pragma unroll
     for (int j = kSeg - 1; j >= 0; --j) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        own.b[k] = f[j][k] * (e[j][k] + own.b[k]);
-        own.a[k] *= f[j][k];
-      }
+      own.b = f[j] * (e[j] + own.b);
+      own.a = own.a * f[j];
     }
-    float G[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) G[k] = carry[k];
-    exchange(p, at, turn, own, G, carry);
+    F<V> G = exchange(p, at, turn, own, carry);
 #pragma unroll
     for (int j = kSeg - 1; j >= 0; --j) {
+      to -= p.d_st;
+      const bool in = t0 + j < at.len;
+      const F<V> dc = e[j] + G;
+      G = f[j] * dc;
+      const Vec<T, V> di = narrow<T, V>(dc * wi[j], in), df = narrow<T, V>(dc * wf[j], in),
+                      dgg = narrow<T, V>(dc * wg[j], in);
       if (at.live && t0 + j < p.T) {
-        const bool in = t0 + j < at.len;
-        Vec<T, V> di = zero, df = zero, dgg = zero;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          if (in) {
-            const float dc = e[j][k] + G[k];
-            G[k] = f[j][k] * dc;
-            di.v[k] = from_f32<T>(dc * wi[j][k]);
-            df.v[k] = from_f32<T>(dc * wf[j][k]);
-            dgg.v[k] = from_f32<T>(dc * wg[j][k]);
-          }
-        }
-        T* to = dg + (t0 + j) * p.d_st;
         store_vec<T, V>(to, di);
         store_vec<T, V>(to + p.H, df);
         store_vec<T, V>(to + 2 * (int64_t)p.H, dgg);
@@ -336,12 +452,9 @@ __global__ void __launch_bounds__(kMaxThreads) scan_backward_kernel(const __grid
   if (!at.live) return;
   for (int64_t t = (int64_t)turns * tile + at.rank * p.seg + at.seg; t < p.T; t += p.seg * cluster) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) store_vec<T, V>(dg + t * p.d_st + (int64_t)q * p.H, zero);
+    for (int q = 0; q < 4; ++q) store_vec<T, V>(dg + t * p.d_st + (int64_t)q * p.H, constant_vec<T, V>(0));
   }
-  if (p.dc0 != nullptr && at.rank == 0 && at.seg == 0) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) p.dc0[(int64_t)at.b * p.H + at.ch + k] = carry[k];
-  }
+  if (p.dc0 != nullptr && at.rank == 0 && at.seg == 0) store_state<V>(p.dc0, state_at, carry);
 }
 
 // How the work is split: channel lanes to fill a warp where H allows, then time segments up to

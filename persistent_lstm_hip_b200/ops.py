@@ -13,16 +13,27 @@ steps and rows in place; only a last axis that is not contiguous is copied first
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple, Union
+import functools
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .core import _DTYPES, _ptr, _require_cuda, _stream
+from .core import _DTYPES, _ptr, _require_cuda
 
 _byref = ctypes.byref
+_empty = torch.empty
+_F32 = torch.float32
 _MASK64 = (1 << 64) - 1
+# The current stream's handle without building a torch.cuda.Stream: small calls are host-bound.
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+# What depends on shapes, strides and types alone (checks, descriptors, sizes) is worked out once for
+# each combination and found again by it in these bounded caches.
+_plan = functools.lru_cache(maxsize=512)
 
 
 def _cuda_float(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -36,45 +47,49 @@ def _cuda_float(t: torch.Tensor, name: str) -> torch.Tensor:
     return t if t.dim() == 0 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 # ---- gated scan ------------------------------------------------------------------------------
-def _scan_desc(gates: torch.Tensor, seq_major: bool) -> _lib.ScanDesc:
+class _ScanPlan(NamedTuple):
+    desc: object       # byref of the descriptor
+    state: tuple       # [B, H]
+    h: tuple           # shape of h
+    checkpoints: int   # f32 elements
+    keep: object       # the descriptor
+
+
+@_plan
+def _scan_plan(shape, strides, dtype, index, seq_major, dh_strides=None) -> _ScanPlan:
+    if len(shape) != 3 or shape[2] == 0 or shape[2] % 4:
+        raise ValueError(f"gates must be [B, T, 4H] with H >= 1, got {tuple(shape)}")
     b, t = (1, 0) if seq_major else (0, 1)
-    return _lib.ScanDesc(gates.shape[b], gates.shape[t], gates.shape[2] // 4, _DTYPES[gates.dtype],
-                         gates.device.index, 0, gates.stride(b), gates.stride(t), 0, 0, 0, 0)
+    H = shape[2] // 4
+    h = (shape[0], shape[1], H)
+    h_strides = (shape[1] * H, H, 1) if dh_strides is None else dh_strides
+    d_strides = (shape[1] * 4 * H, 4 * H, 1)
+    d = _lib.ScanDesc(shape[b], shape[t], H, _DTYPES[dtype], index, 0, strides[b], strides[t], h_strides[b],
+                      h_strides[t], d_strides[b], d_strides[t])
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(_lib.load().plstm_gated_scan_checkpoint_size(_byref(d), _byref(nbytes)))
+    return _ScanPlan(_byref(d), (shape[b], H), h, nbytes.value // 4, d)
 
 
-def _scan_strides(d: _lib.ScanDesc, t: torch.Tensor, seq_major: bool, which: str) -> None:
-    b, s = (t.stride(1), t.stride(0)) if seq_major else (t.stride(0), t.stride(1))
-    setattr(d, which + "_batch_stride", b)
-    setattr(d, which + "_time_stride", s)
-
-
-def _scan_forward(gates, c0, lengths, seq_major, keep, c_n=None):
-    lib = _lib.load()
+def _scan_forward(plan, gates, c0, lengths, keep, c_n=None):
     dev = gates.device
-    d = _scan_desc(gates, seq_major)
-    h = torch.empty(gates.shape[0], gates.shape[1], d.hidden, dtype=gates.dtype, device=dev)
-    _scan_strides(d, h, seq_major, "h")
+    h = _empty(plan.h, dtype=gates.dtype, device=dev)
     if c_n is None:
-        c_n = torch.empty(d.batch, d.hidden, dtype=torch.float32, device=dev)
-    ckpt = None
-    if keep:
-        nbytes = ctypes.c_size_t(0)
-        _lib.check(lib.plstm_gated_scan_checkpoint_size(_byref(d), _byref(nbytes)))
-        ckpt = torch.empty(nbytes.value // 4, dtype=torch.float32, device=dev)
-    _lib.check(lib.plstm_gated_scan_forward(_byref(d), _ptr(gates), _ptr(lengths), _ptr(c0), _ptr(h), _ptr(c_n),
-                                            _ptr(ckpt), _stream(dev)))
+        c_n = _empty(plan.state, dtype=_F32, device=dev)
+    ckpt = _empty(plan.checkpoints, dtype=_F32, device=dev) if keep else None
+    rc = _lib.load().plstm_gated_scan_forward(
+        plan.desc, gates.data_ptr(), _ptr(lengths), _ptr(c0), h.data_ptr(), c_n.data_ptr(), _ptr(ckpt),
+        _stream(dev.index))
+    if rc:
+        _lib.check(rc)
     return h, c_n, ckpt
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gates, c0, lengths, seq_major):
-        h, c_n, ckpt = _scan_forward(gates, c0, lengths, seq_major, True)
+    def forward(ctx, gates, c0, lengths, plan, seq_major):
+        h, c_n, ckpt = _scan_forward(plan, gates, c0, lengths, True)
         ctx.save_for_backward(gates, lengths, ckpt)
         ctx.seq_major = seq_major
         ctx.set_materialize_grads(False)
@@ -84,20 +99,21 @@ class _GatedScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh, dc_n):
         gates, lengths, ckpt = ctx.saved_tensors
-        d = _scan_desc(gates, ctx.seq_major)
-        if dh is not None:
-            dh = dh if dh.stride(2) == 1 else dh.contiguous()
-            _scan_strides(d, dh, ctx.seq_major, "h")
+        if dh is not None and dh.stride(2) != 1:
+            dh = dh.contiguous()
         if dc_n is not None:
             dc_n = dc_n.contiguous()
-        dgates = torch.empty(gates.shape, dtype=gates.dtype, device=gates.device)
-        _scan_strides(d, dgates, ctx.seq_major, "dgates")
-        dc0 = torch.empty(d.batch, d.hidden, dtype=torch.float32, device=gates.device) if ctx.needs_input_grad[1] \
-            else None
-        _lib.check(_lib.load().plstm_gated_scan_backward(
-            _byref(d), _ptr(gates), _ptr(lengths), _ptr(ckpt), _ptr(dh), _ptr(dc_n), _ptr(dgates), _ptr(dc0),
-            _stream(gates.device)))
-        return dgates, dc0, None, None
+        dev = gates.device
+        plan = _scan_plan(gates.shape, gates.stride(), gates.dtype, dev.index, ctx.seq_major,
+                          None if dh is None else dh.stride())
+        dgates = _empty(gates.shape, dtype=gates.dtype, device=dev)
+        dc0 = _empty(plan.state, dtype=_F32, device=dev) if ctx.needs_input_grad[1] else None
+        rc = _lib.load().plstm_gated_scan_backward(
+            plan.desc, gates.data_ptr(), _ptr(lengths), ckpt.data_ptr(), _ptr(dh), _ptr(dc_n), dgates.data_ptr(),
+            _ptr(dc0), _stream(dev.index))
+        if rc:
+            _lib.check(rc)
+        return dgates, dc0, None, None, None
 
 
 def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, *,
@@ -111,21 +127,18 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
     layout and c_n [B,H] f32.  Differentiable in gates and c0.
     """
     gates = _cuda_float(gates, "gates")
-    if gates.dim() != 3 or gates.shape[2] == 0 or gates.shape[2] % 4:
-        raise ValueError(f"gates must be [B, T, 4H] with H >= 1, got {tuple(gates.shape)}")
-    B, H = gates.shape[1 if seq_major else 0], gates.shape[2] // 4
+    plan = _scan_plan(gates.shape, gates.stride(), gates.dtype, gates.device.index, seq_major)
     if c0 is not None:
-        c0 = _require_cuda(c0, "c0", gates.device, torch.float32)
-        if c0.shape != (B, H):
-            raise ValueError(f"c0 must be [{B}, {H}], got {tuple(c0.shape)}")
+        c0 = _require_cuda(c0, "c0", gates.device, _F32)
+        if c0.shape != plan.state:
+            raise ValueError(f"c0 must be {list(plan.state)}, got {tuple(c0.shape)}")
     if lengths is not None:
-        if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.shape != (B,):
-            raise ValueError(f"lengths must be an integer tensor [{B}]")
+        if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.shape != plan.state[:1]:
+            raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
         lengths = lengths.to(device=gates.device, dtype=torch.int32).contiguous()
-    if _wants_grad(gates, c0):
-        return _GatedScan.apply(gates, c0, lengths, seq_major)
-    h, c_n, _ = _scan_forward(gates, c0, lengths, seq_major, False)
-    return h, c_n
+    if torch.is_grad_enabled() and (gates.requires_grad or (c0 is not None and c0.requires_grad)):
+        return _GatedScan.apply(gates, c0, lengths, plan, seq_major)
+    return _scan_forward(plan, gates, c0, lengths, False)[:2]
 
 
 def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
@@ -137,20 +150,24 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
     gates = _cuda_float(gates, "gates")
     if gates.dim() != 2:
         raise ValueError(f"gates must be [B, 4H], got {tuple(gates.shape)}")
-    if out_c is None:
+    if torch.is_grad_enabled() and (gates.requires_grad or c.requires_grad):
+        if out_c is not None:
+            raise ValueError("gated_scan_step with out_c is not differentiable; call it without out_c or under "
+                             "no_grad")
         h, c_n = gated_scan(gates[:, None], c)
         return h[:, 0], c_n
-    if _wants_grad(gates, c):
-        raise ValueError("gated_scan_step with out_c is not differentiable; call it without out_c or under no_grad")
-    B, H = gates.shape[0], gates.shape[1] // 4
-    if H < 1 or gates.shape[1] % 4:
-        raise ValueError(f"gates must be [B, 4H] with H >= 1, got {tuple(gates.shape)}")
-    c = _require_cuda(c, "c", gates.device, torch.float32)
-    _require_cuda(out_c, "out_c", gates.device, torch.float32)
-    if c.shape != (B, H) or out_c.shape != (B, H) or not out_c.is_contiguous():
-        raise ValueError(f"c and out_c must be [{B}, {H}], out_c contiguous")
-    h, c_n, _ = _scan_forward(gates[:, None], c, None, False, False, out_c)
-    return h[:, 0], c_n
+    # One step of [1, B, 4H], so that h comes out as [1, B, H] without a view of the gates.
+    shape, strides = gates.shape, gates.stride()
+    plan = _scan_plan((1, *shape), (0, *strides), gates.dtype, gates.device.index, True)
+    c = _require_cuda(c, "c", gates.device, _F32)
+    if c.shape != plan.state:
+        raise ValueError(f"c must be {list(plan.state)}, got {tuple(c.shape)}")
+    if out_c is not None:
+        _require_cuda(out_c, "out_c", gates.device, _F32)
+        if out_c.shape != plan.state or not out_c.is_contiguous():
+            raise ValueError(f"out_c must be {list(plan.state)} and contiguous")
+    h, c_n, _ = _scan_forward(plan, gates, c, None, False, out_c)
+    return h[0], c_n
 
 
 # ---- dropout --------------------------------------------------------------------------------
@@ -168,36 +185,38 @@ def _drop_desc(p: float, seed: Union[int, torch.Tensor], offset: int, device: to
     return _lib.DropoutDesc(p, seed, offset, None)
 
 
-def _dropout(x, p, seed, offset, residual, dtype):
-    y = torch.empty(x.shape, dtype=dtype, device=x.device)
-    _lib.check(_lib.load().plstm_dropout(_byref(_drop_desc(p, seed, offset, x.device)), x.numel(), _ptr(x),
-                                         _DTYPES[x.dtype], _ptr(residual), _ptr(y), _DTYPES[dtype], x.device.index,
-                                         _stream(x.device)))
+def _dropout(x, drop, residual, dtype):
+    dev = x.device
+    y = _empty(x.shape, dtype=dtype, device=dev)
+    rc = _lib.load().plstm_dropout(_byref(drop), x.numel(), x.data_ptr(), _DTYPES[x.dtype], _ptr(residual),
+                                   y.data_ptr(), _DTYPES[dtype], dev.index, _stream(dev.index))
+    if rc:
+        _lib.check(rc)
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        ctx.args = (p, None if isinstance(seed, torch.Tensor) else seed, offset, x.dtype)
-        ctx.save_for_backward(seed if isinstance(seed, torch.Tensor) else None)
-        return _dropout(x, p, seed, offset, residual, x.dtype if residual is None else residual.dtype)
+    def forward(ctx, x, residual, drop, seed):
+        ctx.args = (drop, x.dtype)
+        # A tensor seed is kept with its version: changing it before the backward is an error.
+        ctx.save_for_backward(seed)
+        return _dropout(x, drop, residual, x.dtype if residual is None else residual.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        p, seed, offset, dtype = ctx.args
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _dropout(dy.contiguous(), p, ctx.saved_tensors[0] if seed is None else seed, offset, None, dtype)
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        drop, dtype = ctx.args
+        ctx.saved_tensors
+        dx = _dropout(dy.contiguous(), drop, None, dtype) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None
 
 
 def _check_residual(residual: torch.Tensor, x: torch.Tensor) -> None:
     if residual.device != x.device or residual.shape != x.shape:
         raise ValueError(f"residual must be {tuple(x.shape)} on {x.device}, got {tuple(residual.shape)} on "
                          f"{residual.device}")
-    if residual.dtype not in (x.dtype, torch.float32):
+    if residual.dtype is not x.dtype and residual.dtype is not _F32:
         raise ValueError(f"residual must be {x.dtype} or float32, got {residual.dtype}")
 
 
@@ -216,12 +235,22 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
     if residual is not None:
         residual = _cuda_float(residual, "residual").contiguous()
         _check_residual(residual, x)
-    if _wants_grad(x, residual):
-        return _Dropout.apply(x, residual, p, seed, offset)
-    return _dropout(x, p, seed, offset, residual, x.dtype if residual is None else residual.dtype)
+    drop = _drop_desc(p, seed, offset, x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, drop, seed if isinstance(seed, torch.Tensor) else None)
+    return _dropout(x, drop, residual, x.dtype if residual is None else residual.dtype)
 
 
 # ---- layer norm -------------------------------------------------------------------------------
+class _NormPlan(NamedTuple):
+    desc: object      # byref of the descriptor
+    rows: tuple       # [rows, cols]
+    stats: tuple      # [2, rows]
+    workspace: int    # bytes of the backward's workspace
+    w_dtype: object
+    keep: object      # the descriptor
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` as [rows, cols] with contiguous columns (a view wherever the strides allow one)."""
     if t.dim() != 2:
@@ -229,113 +258,126 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _norm_desc(x, z_dtype, w_dtype, eps) -> _lib.NormDesc:
-    return _lib.NormDesc(x.shape[0], x.shape[1], _DTYPES[x.dtype], _DTYPES[z_dtype], _DTYPES[w_dtype],
-                         x.device.index, eps, x.stride(0), 0, 0, 0)
+@_plan
+def _norm_plan(rows, cols, x_dtype, z_dtype, w_dtype, index, eps, x_stride, res_stride, dy_stride=0,
+               dz_stride=0) -> _NormPlan:
+    if not 1 <= cols <= _lib.NORM_MAX_COLS:
+        raise ValueError(f"the last axis must be 1 to {_lib.NORM_MAX_COLS} wide, got {cols}")
+    d = _lib.NormDesc(rows, cols, _DTYPES[x_dtype], _DTYPES[z_dtype], _DTYPES[w_dtype], index, eps, x_stride,
+                      res_stride, dy_stride, dz_stride)
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(_lib.load().plstm_layer_norm_backward_workspace_size(_byref(d), _byref(nbytes)))
+    return _NormPlan(_byref(d), (rows, cols), (2, rows), nbytes.value, w_dtype, d)
 
 
-def _norm_forward(x, residual, weight, bias, eps, drop, keep):
+def _norm_inputs(x, residual, weight, bias, eps):
+    """Checks the arguments; x and residual as rows, contiguous weights, and their plan."""
+    if x.dim() == 0:
+        raise ValueError("x must have at least one axis")
+    cols = x.shape[-1]
+    w_dtype = None
+    if weight is not None:
+        w_dtype = weight.dtype
+        weight = _check_weight(weight, "weight", x, cols)
+    if bias is not None:
+        if w_dtype is not None and bias.dtype is not w_dtype:
+            raise ValueError("weight and bias must have one dtype")
+        w_dtype = bias.dtype
+        bias = _check_weight(bias, "bias", x, cols)
+    x2 = _rows(x) if cols else x.reshape(0, 0)
+    r2 = None if residual is None else _rows(residual)
+    dtype = x.dtype
+    plan = _norm_plan(x2.shape[0], cols, dtype, dtype if r2 is None else r2.dtype, w_dtype or dtype, x.device.index,
+                      eps, x2.stride(0), 0 if r2 is None else r2.stride(0))
+    return x2, r2, weight, bias, plan
+
+
+def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, cols: int) -> torch.Tensor:
+    if w.dim() != 1 or w.shape[0] != cols or w.device != x.device:
+        raise ValueError(f"{name} must be [{cols}] on {x.device}, got {tuple(w.shape)} on {w.device}")
+    if w.dtype is not x.dtype and w.dtype is not _F32:
+        raise ValueError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
+    return w.contiguous()
+
+
+def _norm_forward(x, residual, weight, bias, plan, drop, keep):
     """x, residual [rows, cols] -> (y, z or None, stats or None)."""
-    lib = _lib.load()
     dev = x.device
-    w_dtype = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
-    d = _norm_desc(x, x.dtype if residual is None else residual.dtype, w_dtype, eps)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    z = None
-    if residual is not None:
-        z = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-        d.residual_stride = residual.stride(0)
-    stats = torch.empty(2, x.shape[0], dtype=torch.float32, device=dev) if keep else None
-    _lib.check(lib.plstm_layer_norm_forward(_byref(d), None if drop is None else _byref(drop), _ptr(x),
-                                            _ptr(residual), _ptr(weight), _ptr(bias), _ptr(z), _ptr(y), _ptr(stats),
-                                            _stream(dev)))
+    y = _empty(plan.rows, dtype=x.dtype, device=dev)
+    z = None if residual is None else _empty(plan.rows, dtype=residual.dtype, device=dev)
+    stats = _empty(plan.stats, dtype=_F32, device=dev) if keep else None
+    rc = _lib.load().plstm_layer_norm_forward(
+        plan.desc, None if drop is None else _byref(drop), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
+        _ptr(z), y.data_ptr(), _ptr(stats), _stream(dev.index))
+    if rc:
+        _lib.check(rc)
     return y, z, stats
 
 
-def _norm_backward(v, weight, stats, dy, dz, eps, drop, x_dtype, w_dtype, need_dx, need_dres, need_dw, need_db):
-    """Gradients of (x, residual, weight, bias); drop is None for the plain norm."""
-    lib = _lib.load()
+def _norm_backward(v, weight, stats, dy, dz, eps, drop, x_dtype, w_dtype, need):
+    """Gradients of (x, residual, weight, bias) as `need` asks; drop is None for the plain norm."""
     dev = v.device
-    fused = drop is not None
-    d = _lib.NormDesc(v.shape[0], v.shape[1], _DTYPES[x_dtype], _DTYPES[v.dtype], _DTYPES[w_dtype], dev.index, eps,
-                      v.stride(0), 0, dy.stride(0), 0 if dz is None else dz.stride(0))
-    dx = torch.empty(v.shape, dtype=x_dtype, device=dev) if need_dx else None
-    dres = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_dres else None
-    dw = torch.empty(v.shape[1], dtype=w_dtype, device=dev) if need_dw else None
-    db = torch.empty(v.shape[1], dtype=w_dtype, device=dev) if need_db else None
-    ws, nbytes = None, ctypes.c_size_t(0)
-    if need_dw or need_db:
-        _lib.check(lib.plstm_layer_norm_backward_workspace_size(_byref(d), _byref(nbytes)))
-        ws = torch.empty(max(nbytes.value, 16), dtype=torch.uint8, device=dev)
-    _lib.check(lib.plstm_layer_norm_backward(_byref(d), _byref(drop) if fused else None, 1 if fused else 0, _ptr(dy),
-                                             _ptr(dz), _ptr(v), _ptr(weight), _ptr(stats), _ptr(dx), _ptr(dres),
-                                             _ptr(dw), _ptr(db), _ptr(ws), nbytes.value, _stream(dev)))
+    shape = v.shape
+    rows, cols = shape
+    plan = _norm_plan(rows, cols, x_dtype, v.dtype, w_dtype, dev.index, eps, v.stride(0), 0, dy.stride(0),
+                      0 if dz is None else dz.stride(0))
+    dx = _empty(shape, dtype=x_dtype, device=dev) if need[0] else None
+    dres = _empty(shape, dtype=v.dtype, device=dev) if need[1] else None
+    dw = _empty(cols, dtype=w_dtype, device=dev) if need[2] else None
+    db = _empty(cols, dtype=w_dtype, device=dev) if need[3] else None
+    ws = _empty(plan.workspace + 16, dtype=torch.uint8, device=dev) if need[2] or need[3] else None
+    rc = _lib.load().plstm_layer_norm_backward(
+        plan.desc, None if drop is None else _byref(drop), drop is not None, dy.data_ptr(), _ptr(dz), v.data_ptr(),
+        _ptr(weight), stats.data_ptr(), _ptr(dx), _ptr(dres), _ptr(dw), _ptr(db), _ptr(ws), plan.workspace,
+        _stream(dev.index))
+    if rc:
+        _lib.check(rc)
     return dx, dres, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        rows = _rows(x)
-        y, _, stats = _norm_forward(rows, None, weight, bias, eps, None, True)
+    def forward(ctx, x, weight, bias, rows, plan, eps):
+        y, _, stats = _norm_forward(rows, None, weight, bias, plan, None, True)
         ctx.save_for_backward(rows, weight, stats)
-        ctx.eps, ctx.w_dtype = eps, x.dtype if weight is None and bias is None else \
-            (bias if weight is None else weight).dtype
-        return y.view(x.shape)
+        ctx.args = (eps, plan.w_dtype)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
+        eps, w_dtype = ctx.args
         need = ctx.needs_input_grad
-        dx, _, dw, db = _norm_backward(x, weight, stats, _rows(dy), None, ctx.eps, None, x.dtype, ctx.w_dtype,
-                                       need[0], False, need[1], need[2])
-        return None if dx is None else dx.view(dy.shape), dw, db, None
+        dx, _, dw, db = _norm_backward(x, weight, stats, _rows(dy), None, eps, None, x.dtype, w_dtype,
+                                       (need[0], False, need[1], need[2]))
+        return dx if dx is None or dy.dim() == 2 else dx.view(dy.shape), dw, db, None, None, None
 
 
 class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, weight, bias, p, seed, offset, eps):
-        y, z, stats = _norm_forward(_rows(x), _rows(residual), weight, bias, eps,
-                                    _drop_desc(p, seed, offset, x.device), True)
-        ctx.save_for_backward(z, weight, stats, seed if isinstance(seed, torch.Tensor) else None)
-        ctx.args = (p, None if isinstance(seed, torch.Tensor) else seed, offset, eps)
-        ctx.x_dtype = x.dtype
-        ctx.w_dtype = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+    def forward(ctx, x, residual, weight, bias, x2, r2, plan, drop, seed, eps):
+        y, z, stats = _norm_forward(x2, r2, weight, bias, plan, drop, True)
+        ctx.save_for_backward(z, weight, stats, seed)
+        ctx.args = (drop, eps, x.dtype, plan.w_dtype)
         ctx.set_materialize_grads(False)
-        return y.view(x.shape), z.view(x.shape)
+        return (y, z) if x.dim() == 2 else (y.view(x.shape), z.view(x.shape))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dz):
-        z, weight, stats, seed_t = ctx.saved_tensors
-        p, seed, offset, eps = ctx.args
+        z, weight, stats, _ = ctx.saved_tensors
+        drop, eps, x_dtype, w_dtype = ctx.args
         if dy is None and dz is None:
-            return (None,) * 8
+            return (None,) * 10
         shape = (dz if dy is None else dy).shape
-        drop = _drop_desc(p, seed_t if seed is None else seed, offset, z.device)
-        dy = torch.zeros((1, z.shape[1]), dtype=ctx.x_dtype, device=z.device).expand(z.shape) if dy is None \
-            else _rows(dy)
-        need = ctx.needs_input_grad
-        dx, dres, dw, db = _norm_backward(z, weight, stats, dy, None if dz is None else _rows(dz), eps, drop,
-                                          ctx.x_dtype, ctx.w_dtype, need[0], need[1], need[2], need[3])
-        return (None if dx is None else dx.view(shape), None if dres is None else dres.view(shape), dw, db, None,
-                None, None, None)
-
-
-def _check_norm(x: torch.Tensor, weight, bias):
-    if x.dim() == 0 or not 1 <= x.shape[-1] <= _lib.NORM_MAX_COLS:
-        raise ValueError(f"the last axis must be 1 to {_lib.NORM_MAX_COLS} wide, got shape {tuple(x.shape)}")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.device != x.device or t.shape != x.shape[-1:]:
-            raise ValueError(f"{name} must be [{x.shape[-1]}] on {x.device}, got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"{name} must be {x.dtype} or float32, got {t.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one dtype")
-    return (None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous())
+        dy = torch.zeros((1, z.shape[1]), dtype=x_dtype, device=z.device).expand(z.shape) if dy is None else _rows(dy)
+        dx, dres, dw, db = _norm_backward(z, weight, stats, dy, None if dz is None else _rows(dz), eps, drop, x_dtype,
+                                          w_dtype, ctx.needs_input_grad)
+        if len(shape) != 2:
+            dx = None if dx is None else dx.view(shape)
+            dres = None if dres is None else dres.view(shape)
+        return dx, dres, dw, db, None, None, None, None, None, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -346,10 +388,12 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     are f32.  Differentiable in x, weight and bias.
     """
     x = _cuda_float(x, "x")
-    weight, bias = _check_norm(x, weight, bias)
-    if _wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return _norm_forward(_rows(x), None, weight, bias, eps, None, False)[0].view(x.shape)
+    rows, _, weight, bias, plan = _norm_inputs(x, None, weight, bias, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, rows.detach(), plan, eps)
+    y = _norm_forward(rows, None, weight, bias, plan, None, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -365,9 +409,12 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
     x = _cuda_float(x, "x")
     residual = _cuda_float(residual, "residual")
     _check_residual(residual, x)
-    weight, bias = _check_norm(x, weight, bias)
-    if _wants_grad(x, residual, weight, bias):
-        return _DropoutAddLayerNorm.apply(x, residual, weight, bias, p, seed, offset, eps)
-    y, z, _ = _norm_forward(_rows(x), _rows(residual), weight, bias, eps, _drop_desc(p, seed, offset, x.device),
-                            False)
-    return y.view(x.shape), z.view(x.shape)
+    x2, r2, weight, bias, plan = _norm_inputs(x, residual, weight, bias, eps)
+    drop = _drop_desc(p, seed, offset, x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
+                                    (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _DropoutAddLayerNorm.apply(x, residual, weight, bias, x2.detach(), r2.detach(), plan, drop,
+                                          seed if isinstance(seed, torch.Tensor) else None, eps)
+    y, z, _ = _norm_forward(x2, r2, weight, bias, plan, drop, False)
+    return (y, z) if x.dim() == 2 else (y.view(x.shape), z.view(x.shape))

@@ -14,75 +14,86 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// E elements per thread and step (4 or 8), whole vectors; the last n % E elements one by one.
-template <typename TX, typename TY, int E, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(Drop d, int64_t n, const TX* __restrict__ x,
-                                                           const TY* __restrict__ residual, TY* __restrict__ y) {
-  const uint64_t seed = drop_seed(d);
-  const int64_t groups = (n + E - 1) / E;
-  for (int64_t g = blockIdx.x * (int64_t)kThreads + threadIdx.x; g < groups; g += (int64_t)gridDim.x * kThreads) {
-    const int64_t e = g * E;
-    float v[E], r[E];
-    const bool whole = ALIGNED && e + E <= n;
-    if (whole) {
-      constexpr int VX = 16 / sizeof(TX) < E ? 16 / sizeof(TX) : E, VY = 16 / sizeof(TY) < E ? 16 / sizeof(TY) : E;
+// A thread takes kUnroll groups of eight elements a turn, a CTA's apart, and issues all their loads
+// before it draws: with one 16-byte load in flight a thread the kernel waited on memory
+// (82 us for 65.5 M f16 elements, floor 40).
+constexpr int kUnroll = 4;
+
+template <typename T>
+struct Eight {
+  static constexpr int P = 16 / (int)sizeof(T);
+  Vec<T, P> p[8 / P];
+  __device__ __forceinline__ void load(const T* from) {
 #pragma unroll
-      for (int k = 0; k < E; k += VX) {
-        const Vec<TX, VX> in = load_vec<TX, VX>(x + e + k);
+    for (int q = 0; q < 8 / P; ++q) p[q] = load_vec<T, P>(from + q * P);
+  }
+  __device__ __forceinline__ float get(int k) const { return p[k / P].get(k % P); }
+  __device__ __forceinline__ void store(T* to, const float (&f)[8]) {
 #pragma unroll
-        for (int j = 0; j < VX; ++j) v[k + j] = in.get(j);
+    for (int q = 0; q < 8 / P; ++q) {
+      float part[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k) part[k] = f[q * P + k];
+      p[q].set(part);
+      store_vec<T, P>(to + q * P, p[q]);
+    }
+  }
+};
+
+// ALIGNED: all pointers are 16-byte aligned; else, and in the last n % 8 elements, one by one.
+template <typename TX, typename TY, bool RESIDUAL, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, 4) dropout_kernel(Drop d, int64_t n, const TX* __restrict__ x,
+                                                              const TY* __restrict__ residual, TY* __restrict__ y) {
+  const uint64_t seed = uniform_seed(d);
+  const int64_t groups = (n + 7) / 8, whole = ALIGNED ? n / 8 : 0;
+  for (int64_t base = blockIdx.x * (int64_t)(kThreads * kUnroll) + threadIdx.x; base < groups;
+       base += (int64_t)gridDim.x * (kThreads * kUnroll)) {
+    Eight<TX> in[kUnroll];
+    Eight<TY> res[RESIDUAL ? kUnroll : 1];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t g = base + u * kThreads;
+      if (g < whole) {
+        in[u].load(x + g * 8);
+        if constexpr (RESIDUAL) res[u].load(residual + g * 8);
       }
-      if (residual != nullptr) {
+    }
 #pragma unroll
-        for (int k = 0; k < E; k += VY) {
-          const Vec<TY, VY> in = load_vec<TY, VY>(residual + e + k);
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t g = base + u * kThreads, e = g * 8;
+      float v[8];
+      if (g < whole) {
 #pragma unroll
-          for (int j = 0; j < VY; ++j) r[k + j] = in.get(j);
+        for (int k = 0; k < 8; ++k) v[k] = in[u].get(k);
+        drop_vec<8>(d, seed, e, v);
+        if constexpr (RESIDUAL) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(res[u].get(k), v[k]);
+        }
+        Eight<TY> out;
+        out.store(y + e, v);
+      } else if (g < groups) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = e + k < n ? to_f32(x[e + k]) : 0.0f;
+        drop_vec<8>(d, seed, e, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (e + k < n) y[e + k] = from_f32<TY>(RESIDUAL ? __fadd_rn(to_f32(residual[e + k]), v[k]) : v[k]);
         }
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < E; ++k) {
-        const bool in = e + k < n;
-        v[k] = in ? to_f32(x[e + k]) : 0.0f;
-        r[k] = in && residual != nullptr ? to_f32(residual[e + k]) : 0.0f;
-      }
-    }
-    drop_vec<E>(d, seed, e, v);
-    if (residual != nullptr) {
-#pragma unroll
-      for (int k = 0; k < E; ++k) v[k] = __fadd_rn(r[k], v[k]);
-    }
-    if (whole) {
-      constexpr int VY = 16 / sizeof(TY) < E ? 16 / sizeof(TY) : E;
-#pragma unroll
-      for (int k = 0; k < E; k += VY) {
-        float part[VY];
-#pragma unroll
-        for (int j = 0; j < VY; ++j) part[j] = v[k + j];
-        Vec<TY, VY> out;
-        out.set(part);
-        store_vec<TY, VY>(y + e + k, out);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (e + k < n) y[e + k] = from_f32<TY>(v[k]);
     }
   }
 }
 
 template <typename TX, typename TY>
 int32_t launch(const Drop& d, int64_t n, const void* x, const void* residual, void* y, cudaStream_t s) {
-  constexpr int E = sizeof(TX) == 2 || sizeof(TY) == 2 ? 8 : 4;
-  const int64_t groups = (n + E - 1) / E;
-  const int grid = (int)std::min<int64_t>((groups + kThreads - 1) / kThreads, kSMs * 8);
-  if (aligned16(x) && aligned16(y) && aligned16(residual))
-    dropout_kernel<TX, TY, E, true><<<grid, kThreads, 0, s>>>(
-        d, n, static_cast<const TX*>(x), static_cast<const TY*>(residual), static_cast<TY*>(y));
-  else
-    dropout_kernel<TX, TY, E, false><<<grid, kThreads, 0, s>>>(
-        d, n, static_cast<const TX*>(x), static_cast<const TY*>(residual), static_cast<TY*>(y));
+  const int64_t turns = ((n + 7) / 8 + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+  const int grid = (int)std::min<int64_t>(turns, kSMs * 4);
+  const bool aligned = aligned16(x) && aligned16(y) && aligned16(residual);
+  const auto kernel = residual != nullptr ? (aligned ? dropout_kernel<TX, TY, true, true> : dropout_kernel<TX, TY, true, false>)
+                                          : (aligned ? dropout_kernel<TX, TY, false, true> : dropout_kernel<TX, TY, false, false>);
+  kernel<<<grid, kThreads, 0, s>>>(d, n, static_cast<const TX*>(x), static_cast<const TY*>(residual),
+                                   static_cast<TY*>(y));
   PLSTM_TRY_CUDA(cudaGetLastError());
   note_launches(1);
   return PLSTM_OK;

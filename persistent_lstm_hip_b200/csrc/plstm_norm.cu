@@ -8,6 +8,8 @@
 // The weight gradients are summed per thread over the rows its CTA visits, then over the
 // CTA's row groups, then over the CTAs by a second kernel: a fixed order, no atomics.
 #include <algorithm>
+#include <atomic>
+#include <initializer_list>
 
 #include "plstm_ops.cuh"
 
@@ -15,24 +17,37 @@ namespace plstm {
 namespace ops {
 namespace {
 
-constexpr int kGroupThreads = 256;  // CTA size when a row takes at most one warp
-
-// The widest CTA make_split gives a variant: 16384 columns in chunks of 8 x 4 or of 4 x 4 and less.
-constexpr int max_threads(int v) { return v == 8 ? 512 : 1024; }
-
-// How a row of N elements is spread over threads: `tpr` threads take chunks of V elements,
-// chunk c of thread t starting at column (c * tpr + t) * V; a thread has CH chunks.
+// How the work is spread.  Memory is walked in chunks of eight elements that are aligned in the
+// flattened tensor, whatever the row length: a row then starts and ends inside a chunk (its phase
+// is row * cols mod 8), whose foreign elements are masked, every other access is 16 bytes wide, and a
+// chunk is two whole Philox blocks.  A team of `tpr` threads (a power of two up to a warp, or whole
+// warps) takes a row: chunk c of lane t is the row's (c * tpr + t)-th.  A CTA holds `teams` teams.
+// The forward issues the loads of a team's next row before the sums over the current one.
+//
+// WHOLE: cols is a multiple of 8 and every row is aligned, so there is no phase and no mask.
 struct Split {
-  int v, ch, tpr, block;
+  int ch, tpr, teams;
+  int block() const { return tpr * teams; }
+};
+// Widest team: four chunks a thread hold 16384 columns (2049 chunks), two a thread 4096 (513).
+constexpr int max_block(int ch) { return ch == 4 ? 544 : 288; }
+constexpr int kTeamBlock = 128;  // CTA size up to which teams share a CTA
+
+// A tensor as the kernels address it: element (row, col) at row * stride + col.
+struct Mat {
+  const void* p;
+  int64_t stride;
+  int64_t extent;  // elements from the first to the last, so that no vector leaves the tensor
+  int vec;         // chunks are 16-byte aligned
 };
 
 struct NormArgs {
   int64_t rows;
-  int cols, tpr;
+  int cols, tpr, teams;
   float eps;
-  int64_t x_stride, res_stride, dy_stride, dz_stride;
-  const void *x, *residual, *dy, *dz, *v, *weight, *bias;
-  void *z, *y, *dx, *dres;
+  Mat x, residual, z, y;        // forward
+  Mat dy, dz, v, dx, dres;      // backward
+  const void *weight, *bias;
   float* mean;
   float* rstd;
   float* partial;
@@ -40,265 +55,458 @@ struct NormArgs {
   Drop drop;
 };
 
-// Sum over the `tpr` threads of a row (a power of two up to 32, or the whole CTA).
+// Teams of several warps share a CTA only as two of 64 threads.  The barriers' numbers are constants:
+// a number in a register makes the compiler claim all 16, and then three CTAs fill an SM.
+__device__ __forceinline__ void team_sync(int team, int threads) {
+  if (threads > kTeamBlock / 2) {
+    __syncthreads();
+  } else if (team == 0) {
+    asm volatile("bar.sync 1, 64;" ::: "memory");
+  } else {
+    asm volatile("bar.sync 2, 64;" ::: "memory");
+  }
+}
+
+// Sums NV values over a team.  `scratch` [teams][2][NV][32]: two turns apart, so that one barrier a
+// sum is enough (`turn` alternates from sum to sum).
 template <int NV>
-__device__ __forceinline__ void row_sum(float (&a)[NV], int tpr, float* scratch) {
+__device__ __forceinline__ void team_sum(float (&a)[NV], int team, int tpr, float* scratch, int turn) {
   for (int o = min(tpr, 32) >> 1; o > 0; o >>= 1) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) a[k] += __shfl_xor_sync(0xffffffffu, a[k], o);
   }
   if (tpr <= 32) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = tpr >> 5;
-  __syncthreads();  // the scratch of the previous sum has been read
-  if (lane == 0) {
+  const int t = threadIdx.x - team * tpr, warps = tpr >> 5;
+  float* mine = scratch + (team * 2 + (turn & 1)) * NV * 32;
+  if ((t & 31) == 0) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) scratch[k * 32 + warp] = a[k];
+    for (int k = 0; k < NV; ++k) mine[(t >> 5) * NV + k] = a[k];
   }
-  __syncthreads();
+  team_sync(team, tpr);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    a[k] = lane < warps ? scratch[k * 32 + lane] : 0.0f;
-    for (int o = 16; o > 0; o >>= 1) a[k] += __shfl_xor_sync(0xffffffffu, a[k], o);
+  for (int k = 0; k < NV; ++k) a[k] = 0.0f;
+#pragma unroll 4
+  for (int w = 0; w < warps; ++w) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) a[k] += mine[w * NV + k];
   }
 }
 
-// V elements of a weight that has x's type or f32 (NULL: `none`).  V > 1 needs 16-byte aligned weights.
-template <typename TX, int V>
-__device__ __forceinline__ void load_weight(const void* w, int dtype, int col, float none, float (&out)[V]) {
-  if (w == nullptr) {
+// Eight elements as they lie in memory.
+template <typename T>
+struct Chunk {
+  static constexpr int P = 16 / (int)sizeof(T);
+  Vec<T, P> p[8 / P];
+  __device__ __forceinline__ float get(int k) const { return p[k / P].get(k % P); }
+  __device__ __forceinline__ F<2> pair(int k) const { return F<2>::of(get(2 * k), get(2 * k + 1)); }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) out[k] = none;
-  } else if (sizeof(TX) == 4 || dtype == PLSTM_F32) {
-    constexpr int VW = V < 4 ? V : 4;
+    for (int q = 0; q < 8 / P; ++q) {
+      float part[P];
 #pragma unroll
-    for (int q = 0; q < V; q += VW) {
-      const Vec<float, VW> in = load_vec<float, VW>(static_cast<const float*>(w) + col + q);
-#pragma unroll
-      for (int k = 0; k < VW; ++k) out[q + k] = in.get(k);
+      for (int k = 0; k < P; ++k) part[k] = f[q * P + k];
+      p[q].set(part);
     }
-  } else {
-    const Vec<TX, V> in = load_vec<TX, V>(static_cast<const TX*>(w) + col);
-#pragma unroll
-    for (int k = 0; k < V; ++k) out[k] = in.get(k);
   }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int q = 0; q < 8 / P; ++q) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[q].w[k] = 0;
+    }
+  }
+  // Columns col .. col + 7 of a row of `cols`, those outside it as zero.
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const Mat& m, int64_t row, int col, int cols) {
+    const int64_t at = row * m.stride + col;
+    const T* from = static_cast<const T*>(m.p) + at;
+    if (WHOLE || (m.vec && at >= 0 && at + 8 <= m.extent)) {
+#pragma unroll
+      for (int q = 0; q < 8 / P; ++q) p[q] = load_vec<T, P>(from + q * P);
+      if (!WHOLE && (col < 0 || col + 8 > cols)) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = col + k >= 0 && col + k < cols ? get(k) : 0.0f;
+        set(f);
+      }
+    } else {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = col + k >= 0 && col + k < cols ? to_f32(from[k]) : 0.0f;
+      set(f);
+    }
+  }
+  template <bool WHOLE>
+  __device__ __forceinline__ void store(const Mat& m, int64_t row, int col, int cols) const {
+    T* to = static_cast<T*>(const_cast<void*>(m.p)) + row * m.stride + col;
+    if (WHOLE || (m.vec && col >= 0 && col + 8 <= cols)) {
+#pragma unroll
+      for (int q = 0; q < 8 / P; ++q) store_vec<T, P>(to + q * P, p[q]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col + k >= 0 && col + k < cols) to[k] = from_f32<T>(get(k));
+    }
+  }
+};
+
+// A weight of `cols` columns in shared memory as f32, so that a warp's reads of its chunks meet no
+// bank twice: without phases as 16-byte halves of the chunks, else by column modulo 8.
+__host__ __device__ inline int chunk_columns(int cols) { return (cols + 7) / 8 + 1; }
+template <bool WHOLE>
+struct Columns {
+  float* s;
+  int n;  // chunk_columns(cols)
+  __device__ __forceinline__ int place(int col) const {
+    return WHOLE ? (((col >> 2) & 1) * n + (col >> 3)) * 4 + (col & 3) : (col & 7) * n + (col >> 3);
+  }
+  __device__ __forceinline__ void fill(const void* w, int dtype, int cols, float none) const {
+    for (int i = threadIdx.x; i < 8 * n; i += blockDim.x)
+      s[place(i)] = i >= cols ? 0.0f : w != nullptr ? load_any(w, dtype, i) : none;
+  }
+  __device__ __forceinline__ void read(int col, F<2> (&out)[4]) const {
+    if constexpr (WHOLE) {
+      const float4 lo = reinterpret_cast<const float4*>(s)[col >> 3], hi = reinterpret_cast<const float4*>(s)[n + (col >> 3)];
+      out[0] = F<2>::of(lo.x, lo.y);
+      out[1] = F<2>::of(lo.z, lo.w);
+      out[2] = F<2>::of(hi.x, hi.y);
+      out[3] = F<2>::of(hi.z, hi.w);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = s[place(max(col + k, 0))];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[k] = F<2>::of(f[2 * k], f[2 * k + 1]);
+    }
+  }
+};
+
+// Walks a team over its rows.
+struct Team {
+  int team, lane;
+  int64_t first, step;  // first row of the warp's first team, rows between turns
+  int within;           // this team's place in the warp
+  __device__ __forceinline__ Team(const NormArgs& a) {
+    team = threadIdx.x / a.tpr;
+    lane = threadIdx.x - team * a.tpr;
+    const int head = a.tpr < 32 ? (threadIdx.x & ~31) / a.tpr : team;
+    first = (int64_t)blockIdx.x * a.teams + head;
+    within = team - head;
+    step = (int64_t)gridDim.x * a.teams;
+  }
+};
+// Elements of the row's first chunk that belong to the row before.
+template <bool WHOLE>
+__device__ __forceinline__ int phase_of(int64_t row, int cols) {
+  return WHOLE ? 0 : (int)((uint32_t)row * (uint32_t)cols & 7u);
 }
 
-template <typename TX, typename TZ, int V, int CH, bool FUSED>
-__global__ void __launch_bounds__(max_threads(V)) norm_forward_kernel(NormArgs a) {
-  __shared__ float scratch[64];
-  const int tpr = a.tpr, lane = threadIdx.x % tpr;
-  const int rows_per_cta = blockDim.x / tpr;
-  const uint64_t seed = FUSED ? drop_seed(a.drop) : 0;
-  const float inv_n = 1.0f / (float)a.cols;
-  // Every thread of a warp takes every turn (the sums shuffle over the whole warp).
-  for (int64_t row0 = (int64_t)blockIdx.x * rows_per_cta; row0 < a.rows; row0 += (int64_t)gridDim.x * rows_per_cta) {
-    const int64_t row = row0 + threadIdx.x / tpr;
-    const bool live = row < a.rows;
-    float v[CH][V];
-    float sum[1] = {0.0f};
+template <typename TX, typename TZ, int CH, bool FUSED, bool WHOLE>
+__global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_forward_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float scratch[2 * 32 * (kTeamBlock / 32)];
+  extern __shared__ __align__(16) float columns[];
+  const Team at(a);
+  const int tpr = a.tpr, cols = a.cols, n = chunk_columns(cols);
+  const uint64_t seed = FUSED ? uniform_seed(a.drop) : 0;
+  const float inv_n = 1.0f / (float)cols;
+  Chunk<TX> x[CH];
+  Chunk<TZ> r[FUSED ? CH : 1];
+  const auto fetch = [&](int64_t row) {
+    const int col0 = at.lane * 8 - phase_of<WHOLE>(row, cols);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int col = (c * tpr + lane) * V;
-      if (live && col < a.cols) {
-        const Vec<TX, V> in = load_vec<TX, V>(static_cast<const TX*>(a.x) + row * a.x_stride + col);
+      const int col = col0 + c * tpr * 8;
+      if (row < a.rows && col < cols) {
+        x[c].template load<WHOLE>(a.x, row, col, cols);
+        if constexpr (FUSED) r[c].template load<WHOLE>(a.residual, row, col, cols);
+      }
+    }
+  };
+  fetch(at.first + at.within);
+  const Columns<WHOLE> w{columns, n}, b{columns + 8 * n, n};
+  w.fill(a.weight, a.w_dtype, cols, 1.0f);
+  b.fill(a.bias, a.w_dtype, cols, 0.0f);
+  __syncthreads();
+  for (int64_t head = at.first; head < a.rows; head += at.step) {
+    const int64_t row = head + at.within;
+    const bool live = row < a.rows;
+    const int phase = phase_of<WHOLE>(row, cols), col0 = at.lane * 8 - phase;
+    F<2> v[CH][4], sum2 = F<2>::of(0.0f);
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[c][k] = in.get(k);
+    for (int c = 0; c < CH; ++c) {
+      const int col = col0 + c * tpr * 8;
+      if (live && col < cols) {
         if constexpr (FUSED) {
-          const int64_t e = row * a.cols + col;
-          drop_vec<V>(a.drop, seed, e, v[c]);
-          const TZ* res = static_cast<const TZ*>(a.residual) + row * a.res_stride + col;
-          constexpr int VZ = 16 / sizeof(TZ) < V ? 16 / sizeof(TZ) : V;
+          float f[8];
 #pragma unroll
-          for (int q = 0; q < V; q += VZ) {
-            const Vec<TZ, VZ> r = load_vec<TZ, VZ>(res + q);
-            float part[VZ];
+          for (int k = 0; k < 8; ++k) f[k] = x[c].get(k);
+          drop_vec<8>(a.drop, seed, row * cols + col, f);
 #pragma unroll
-            for (int k = 0; k < VZ; ++k) part[k] = __fadd_rn(r.get(k), v[c][q + k]);
-            Vec<TZ, VZ> z;
-            z.set(part);
+          for (int k = 0; k < 8; ++k) f[k] = __fadd_rn(r[c].get(k), f[k]);
+          r[c].set(f);  // the norm is of z as stored
+          r[c].template store<WHOLE>(a.z, row, col, cols);
+          if (!WHOLE && (col < 0 || col + 8 > cols)) {
 #pragma unroll
-            for (int k = 0; k < VZ; ++k) v[c][q + k] = z.get(k);  // the norm is of z as stored
-            store_vec<TZ, VZ>(static_cast<TZ*>(a.z) + e + q, z);
+            for (int k = 0; k < 8; ++k) f[k] = col + k >= 0 && col + k < cols ? r[c].get(k) : 0.0f;
+            r[c].set(f);
           }
-        }
 #pragma unroll
-        for (int k = 0; k < V; ++k) sum[0] += v[c][k];
+          for (int k = 0; k < 4; ++k) v[c][k] = r[c].pair(k);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[c][k] = x[c].pair(k);
+        }
       } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[c][k] = 0.0f;
+        for (int k = 0; k < 4; ++k) v[c][k] = F<2>::of(0.0f);
       }
+      sum2 = sum2 + ((v[c][0] + v[c][1]) + (v[c][2] + v[c][3]));
     }
-    row_sum<1>(sum, tpr, scratch);
+    fetch(row + at.step);
+    float sum[1] = {sum2.get(0) + sum2.get(1)};
+    team_sum<1>(sum, at.team, tpr, scratch, 0);
     const float mean = sum[0] * inv_n;
-    float sq[1] = {0.0f};
+    F<2> sq2 = F<2>::of(0.0f);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      if ((c * tpr + lane) * V < a.cols) {
+      const int col = col0 + c * tpr * 8;
+      if (col < cols) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          v[c][k] -= mean;
-          sq[0] += v[c][k] * v[c][k];
+        for (int k = 0; k < 4; ++k) v[c][k] = v[c][k] + F<2>::of(-mean);
+        if (!WHOLE && (col < 0 || col + 8 > cols)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[c][k] = F<2>::of(col + 2 * k >= 0 && col + 2 * k < cols ? v[c][k].get(0) : 0.0f,
+                               col + 2 * k + 1 >= 0 && col + 2 * k + 1 < cols ? v[c][k].get(1) : 0.0f);
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sq2 = fma(v[c][k], v[c][k], sq2);
       }
     }
-    row_sum<1>(sq, tpr, scratch);
-    const float rstd = 1.0f / sqrtf(sq[0] * inv_n + a.eps);
+    float sq[1] = {sq2.get(0) + sq2.get(1)};
+    team_sum<1>(sq, at.team, tpr, scratch, 1);
+    const float rstd = rsqrt_rn(sq[0] * inv_n + a.eps);
     if (!live) continue;
-    if (a.mean != nullptr && lane == 0) {
+    if (a.mean != nullptr && at.lane == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int col = (c * tpr + lane) * V;
-      if (col < a.cols) {
-        float w[V], b[V];
-        load_weight<TX, V>(a.weight, a.w_dtype, col, 1.0f, w);
-        load_weight<TX, V>(a.bias, a.w_dtype, col, 0.0f, b);
+      const int col = col0 + c * tpr * 8;
+      if (col < cols) {
+        F<2> ww[4], bb[4];
+        w.read(col, ww);
+        b.read(col, bb);
+        float f[8];
 #pragma unroll
-        for (int k = 0; k < V; ++k) w[k] = v[c][k] * rstd * w[k] + b[k];
-        Vec<TX, V> out;
-        out.set(w);
-        store_vec<TX, V>(static_cast<TX*>(a.y) + row * a.cols + col, out);
+        for (int k = 0; k < 4; ++k) {
+          const F<2> o = fma(v[c][k] * F<2>::of(rstd), ww[k], bb[k]);
+          f[2 * k] = o.get(0);
+          f[2 * k + 1] = o.get(1);
+        }
+        Chunk<TX> out;
+        out.set(f);
+        out.template store<WHOLE>(a.y, row, col, cols);
       }
     }
   }
 }
 
-// TV: the normalised tensor's type (x or z).  partial [gridDim.x][2][cols], or NULL.
-template <typename TX, typename TV, int V, int CH, bool FUSED>
-__global__ void __launch_bounds__(max_threads(V)) norm_backward_kernel(NormArgs a) {
-  extern __shared__ float acc[];  // [2][cols] when a CTA holds several row groups
-  __shared__ float scratch[64];
-  const int tpr = a.tpr, lane = threadIdx.x % tpr;
-  const int rows_per_cta = blockDim.x / tpr;
-  const uint64_t seed = FUSED ? drop_seed(a.drop) : 0;
-  const float inv_n = 1.0f / (float)a.cols;
-  const int64_t v_stride = FUSED ? (int64_t)a.cols : a.x_stride;
-  constexpr int VV = 16 / sizeof(TV) < V ? 16 / sizeof(TV) : V;
-  float dw[CH][V], db[CH][V];
+// TV: the normalised tensor's type (x or z).  partial [gridDim.x][2][cols], or NULL.  A team's rows
+// all have one phase (their distance is a multiple of 8), so a thread's columns stay its own and
+// the sums of the weight gradients stay with it: in registers, or (CH = 4) in shared memory.
+template <typename TX, typename TV, int CH, bool FUSED, bool WHOLE>
+__global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+  constexpr bool REGS = CH < 4;
+  __shared__ float scratch[2 * 2 * 32 * (kTeamBlock / 32)];
+  extern __shared__ __align__(16) float columns[];
+  const Team at(a);
+  const int tpr = a.tpr, cols = a.cols, n = chunk_columns(cols);
+  const uint64_t seed = FUSED ? uniform_seed(a.drop) : 0;
+  const float inv_n = 1.0f / (float)cols;
+  const int col0 = at.lane * 8 - phase_of<WHOLE>(at.first + at.within, cols);
+  // With !REGS [2][CH * 4][tpr] pairs.
+  F<2>* const acc = reinterpret_cast<F<2>*>(columns + 8 * n) + at.lane;
+  F<2> dw[REGS ? CH : 1][4], db[REGS ? CH : 1][4];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) dw[c][k] = db[c][k] = 0.0f;
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (REGS)
+        dw[c][k] = db[c][k] = F<2>::of(0.0f);
+      else
+        acc[(c * 4 + k) * tpr] = acc[((CH + c) * 4 + k) * tpr] = F<2>::of(0.0f);
+    }
   }
-  for (int64_t row0 = (int64_t)blockIdx.x * rows_per_cta; row0 < a.rows; row0 += (int64_t)gridDim.x * rows_per_cta) {
-    const int64_t row = row0 + threadIdx.x / tpr;
-    const bool live = row < a.rows;
-    float xh[CH][V], g[CH][V];
-    float s[2] = {0.0f, 0.0f};
-    const float mean = live ? a.mean[row] : 0.0f, rstd = live ? a.rstd[row] : 0.0f;
+  // Rows are fetched a turn ahead where the registers hold two (CH = 1).
+  constexpr bool AHEAD = CH == 1;
+  Chunk<TX> next_dy[AHEAD ? CH : 1];
+  Chunk<TV> next_in[AHEAD ? CH : 1];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  const auto fetch = [&](int64_t row, Chunk<TX>* dy, Chunk<TV>* in, float& mean, float& rstd) {
+    if (row >= a.rows) return;
+    mean = a.mean[row];
+    rstd = a.rstd[row];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int col = (c * tpr + lane) * V;
-      if (live && col < a.cols) {
-        const Vec<TX, V> dy = load_vec<TX, V>(static_cast<const TX*>(a.dy) + row * a.dy_stride + col);
+      const int col = col0 + c * tpr * 8;
+      if (col < cols) {
+        dy[c].template load<WHOLE>(a.dy, row, col, cols);
+        in[c].template load<WHOLE>(a.v, row, col, cols);
+      }
+    }
+  };
+  if constexpr (AHEAD) fetch(at.first + at.within, next_dy, next_in, next_mean, next_rstd);
+  const Columns<WHOLE> w{columns, n};
+  w.fill(a.weight, a.w_dtype, cols, 1.0f);
+  __syncthreads();
+  F<2> ww[4];
+  if (AHEAD && col0 < cols) w.read(col0, ww);
+  int turn = 0;
+  for (int64_t head = at.first; head < a.rows; head += at.step, ++turn) {
+    const int64_t row = head + at.within;
+    const bool live = row < a.rows;
+    Chunk<TX> dy[CH];
+    Chunk<TV> in[CH], dz[FUSED ? CH : 1];
+    float mean = 0.0f, rstd = 0.0f;
+    if constexpr (AHEAD) {
+      dy[0] = next_dy[0];
+      in[0] = next_in[0];
+      mean = next_mean;
+      rstd = next_rstd;
+      fetch(row + at.step, next_dy, next_in, next_mean, next_rstd);
+    } else {
+      fetch(row, dy, in, mean, rstd);
+    }
+    if constexpr (FUSED) {
 #pragma unroll
-        for (int q = 0; q < V; q += VV) {
-          const Vec<TV, VV> in = load_vec<TV, VV>(static_cast<const TV*>(a.v) + row * v_stride + col + q);
+      for (int c = 0; c < CH; ++c) {
+        const int col = col0 + c * tpr * 8;
+        if (live && col < cols && a.dz.p != nullptr) dz[c].template load<WHOLE>(a.dz, row, col, cols);
+      }
+    }
+    const F<2> scale = F<2>::of(rstd), shift = F<2>::of(-mean);
+    F<2> s0 = F<2>::of(0.0f), s1 = s0;
 #pragma unroll
-          for (int k = 0; k < VV; ++k) xh[c][q + k] = (in.get(k) - mean) * rstd;
-        }
-        float w[V];
-        load_weight<TX, V>(a.weight, a.w_dtype, col, 1.0f, w);
+    for (int c = 0; c < CH; ++c) {
+      const int col = col0 + c * tpr * 8;
+      if (live && col < cols) {
+        if constexpr (!AHEAD) w.read(col, ww);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = dy.get(k);
-          dw[c][k] += d * xh[c][k];
-          db[c][k] += d;
-          g[c][k] = d * w[k];
-          s[0] += g[c][k];
-          s[1] += g[c][k] * xh[c][k];
+        for (int k = 0; k < 4; ++k) {
+          // dy is zero outside the row, and so is every sum's term there.
+          const F<2> d = dy[c].pair(k), xh = (in[c].pair(k) + shift) * scale, g = d * ww[k];
+          s0 = s0 + g;
+          s1 = fma(g, xh, s1);
+          if constexpr (REGS) {
+            dw[c][k] = fma(d, xh, dw[c][k]);
+            db[c][k] = db[c][k] + d;
+          } else {
+            F<2>&aw = acc[(c * 4 + k) * tpr], &ab = acc[((CH + c) * 4 + k) * tpr];
+            aw = fma(d, xh, aw);
+            ab = ab + d;
+          }
         }
       }
     }
-    row_sum<2>(s, tpr, scratch);
+    float s[2] = {s0.get(0) + s0.get(1), s1.get(0) + s1.get(1)};
+    team_sum<2>(s, at.team, tpr, scratch, turn);
     if (!live) continue;
-    const float m1 = s[0] * inv_n, m2 = s[1] * inv_n;
+    const F<2> m1 = F<2>::of(-s[0] * inv_n), m2 = F<2>::of(-s[1] * inv_n);
+    // xh and g once more from what was read, instead of two more f32 values an element kept.
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int col = (c * tpr + lane) * V;
-      if (col < a.cols) {
-        const int64_t e = row * a.cols + col;
-        float dv[V];
+      const int col = col0 + c * tpr * 8;
+      if (col < cols) {
+        if constexpr (!AHEAD) w.read(col, ww);
+        float dv[8];
 #pragma unroll
-        for (int k = 0; k < V; ++k) dv[k] = rstd * (g[c][k] - m1 - xh[c][k] * m2);
-        if constexpr (FUSED) {
-          if (a.dz != nullptr) {
-#pragma unroll
-            for (int q = 0; q < V; q += VV) {
-              const Vec<TV, VV> dz = load_vec<TV, VV>(static_cast<const TV*>(a.dz) + row * a.dz_stride + col + q);
-#pragma unroll
-              for (int k = 0; k < VV; ++k) dv[q + k] += dz.get(k);
-            }
+        for (int k = 0; k < 4; ++k) {
+          const F<2> xh = (in[c].pair(k) + shift) * scale;
+          F<2> o = fma(xh, m2, fma(dy[c].pair(k), ww[k], m1)) * scale;
+          if constexpr (FUSED) {
+            if (a.dz.p != nullptr) o = o + dz[c].pair(k);
           }
-          if (a.dres != nullptr) {
-#pragma unroll
-            for (int q = 0; q < V; q += VV) {
-              float part[VV];
-#pragma unroll
-              for (int k = 0; k < VV; ++k) part[k] = dv[q + k];
-              Vec<TV, VV> out;
-              out.set(part);
-              store_vec<TV, VV>(static_cast<TV*>(a.dres) + e + q, out);
-            }
-          }
-          if (a.dx == nullptr) continue;
-          drop_vec<V>(a.drop, seed, e, dv);
+          dv[2 * k] = o.get(0);
+          dv[2 * k + 1] = o.get(1);
         }
-        if (a.dx != nullptr) {
-          Vec<TX, V> out;
+        if constexpr (FUSED) {
+          if (a.dres.p != nullptr) {
+            Chunk<TV> out;
+            out.set(dv);
+            out.template store<WHOLE>(a.dres, row, col, cols);
+          }
+          if (a.dx.p == nullptr) continue;
+          drop_vec<8>(a.drop, seed, row * cols + col, dv);
+        }
+        if (a.dx.p != nullptr) {
+          Chunk<TX> out;
           out.set(dv);
-          store_vec<TX, V>(static_cast<TX*>(a.dx) + e, out);
+          out.template store<WHOLE>(a.dx, row, col, cols);
         }
       }
     }
   }
   if (a.partial == nullptr) return;
-  float* to = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
-  if (tpr >= 32 && rows_per_cta == 1) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int col = (c * tpr + lane) * V;
-      if (col < a.cols) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          to[col + k] = dw[c][k];
-          to[a.cols + col + k] = db[c][k];
-        }
-      }
-    }
-    return;
-  }
-  // Row groups within a warp, then the warps one after the other.
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      for (int o = tpr; o < 32; o <<= 1) {
-        dw[c][k] += __shfl_xor_sync(0xffffffffu, dw[c][k], o);
-        db[c][k] += __shfl_xor_sync(0xffffffffu, db[c][k], o);
-      }
-    }
-  }
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  for (int w = 0; w < warps; ++w) {
-    if (warp == w && (int)(threadIdx.x & 31) < tpr) {
+  float* to = a.partial + (int64_t)blockIdx.x * 2 * cols;
+  if constexpr (REGS) {
+    // Teams of a warp that share a phase, then whatever is left one after the other.
+    int together = 1;  // teams summed by shuffles
+    if (WHOLE && tpr < 32) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int col = (c * tpr + lane) * V;
-        if (col < a.cols) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            acc[col + k] = (w > 0 ? acc[col + k] : 0.0f) + dw[c][k];
-            acc[a.cols + col + k] = (w > 0 ? acc[a.cols + col + k] : 0.0f) + db[c][k];
+        for (int k = 0; k < 4; ++k) {
+          float f[4] = {dw[c][k].get(0), dw[c][k].get(1), db[c][k].get(0), db[c][k].get(1)};
+          for (int o = tpr; o < 32; o <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] += __shfl_xor_sync(0xffffffffu, f[i], o);
+          }
+          dw[c][k] = F<2>::of(f[0], f[1]);
+          db[c][k] = F<2>::of(f[2], f[3]);
+        }
+      }
+      together = 32 / tpr;
+    }
+    // The sums take the weight's place: [2][8 n] in its layout.
+    __syncthreads();
+    const Columns<WHOLE> sums[2] = {{columns, n}, {columns + 8 * n, n}};
+    for (int i = threadIdx.x; i < 16 * n; i += blockDim.x) columns[i] = 0.0f;
+    __syncthreads();
+    for (int u = 0; u < a.teams; u += together) {
+      if (at.team == u) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int col = col0 + c * tpr * 8;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (col + k >= 0 && col + k < cols) {
+              sums[0].s[sums[0].place(col + k)] += dw[c][k >> 1].get(k & 1);
+              sums[1].s[sums[1].place(col + k)] += db[c][k >> 1].get(k & 1);
+            }
           }
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) {
+      const int which = i >= cols ? 1 : 0, col = i - which * cols;
+      to[i] = sums[which].s[sums[which].place(col)];
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = col0 + c * tpr * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (col + k >= 0 && col + k < cols) {
+          to[col + k] = acc[(c * 4 + k / 2) * tpr].get(k & 1);
+          to[cols + col + k] = acc[((CH + c) * 4 + k / 2) * tpr].get(k & 1);
+        }
+      }
+    }
   }
-  for (int i = threadIdx.x; i < 2 * a.cols; i += blockDim.x) to[i] = acc[i];
 }
 
 // dweight / dbias from the CTAs' partial sums [parts][2][cols]: 32 columns per CTA, 32 threads
@@ -319,78 +527,115 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __r
   if (threadIdx.x == 0 && c < cols && out != nullptr) store_any(out, w_dtype, c, s);
 }
 
-// Vectors of 16 bytes of x where every row allows them, else single elements.
-Split make_split(const plstm_norm_desc& d, bool vec_ok) {
+// Chunks a thread takes: enough to spread a row's fixed costs (sums, barriers, square root) over,
+// as far as the registers hold them.
+Split make_split(const plstm_norm_desc& d, bool whole, bool backward) {
   Split s;
-  s.v = vec_ok ? 16 / (int)dtype_size(d.x_dtype) : 1;
-  const int chunks = (d.cols + s.v - 1) / s.v;
-  s.tpr = 1;
-  while (s.tpr < 32 && s.tpr < chunks) s.tpr *= 2;
-  s.ch = 1;
-  while (s.ch < 4 && s.ch * s.tpr < chunks) s.ch *= 2;
-  while (s.tpr < 1024 && s.ch * s.tpr < chunks) s.tpr *= 2;
-  if (s.ch * s.tpr < chunks) s.ch = 16;  // single elements, more than 4096 columns
-  s.block = s.tpr <= 32 ? kGroupThreads : s.tpr;
+  const int chunks = whole ? d.cols / 8 : chunk_columns(d.cols);
+  const bool f32 = d.x_dtype == PLSTM_F32;
+  s.ch = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
+  if (f32 && chunks <= 513) s.ch = std::min(s.ch, 2);
+  if (backward) s.ch = chunks <= 257 ? 1 : chunks <= 513 ? 2 : 4;
+  const int threads = (chunks + s.ch - 1) / s.ch;
+  if (threads >= 32) {
+    s.tpr = (threads + 31) / 32 * 32;
+  } else {
+    s.tpr = 1;
+    while (s.tpr < threads) s.tpr *= 2;
+  }
+  s.teams = std::max(1, kTeamBlock / s.tpr);
   return s;
 }
 
-int64_t row_ctas(const plstm_norm_desc& d, const Split& s, int per_sm) {
-  const int64_t per_cta = s.block / s.tpr;
-  return std::min<int64_t>((d.rows + per_cta - 1) / per_cta, (int64_t)kSMs * per_sm);
+size_t forward_smem(const plstm_norm_desc& d) { return (size_t)16 * chunk_columns(d.cols) * sizeof(float); }
+size_t backward_smem(const plstm_norm_desc& d, const Split& s) {
+  const size_t n = chunk_columns(d.cols);
+  return (s.ch < 4 ? 16 * n : 8 * n + (size_t)2 * 8 * s.ch * s.tpr) * sizeof(float);
 }
 
-int backward_per_sm(const Split& s) { return s.block >= 1024 ? 1 : s.block >= 512 ? 2 : s.block == 256 ? 2 : 4; }
+// CTAs of a launch: what the rows need, at most as many as are resident at once (`per_sm` an SM), so
+// that no second wave of a few CTAs follows the first.  The backward's rows a turn are a multiple of 8.
+int64_t forward_ctas(const plstm_norm_desc& d, const Split& s, int per_sm) {
+  return std::min<int64_t>((d.rows + s.teams - 1) / s.teams, (int64_t)kSMs * per_sm);
+}
+int64_t backward_ctas(const plstm_norm_desc& d, const Split& s, int per_sm) {
+  const int64_t unit = 8 / std::min(8, s.teams & -s.teams);  // CTAs whose teams are a multiple of 8
+  const int64_t need = ((d.rows + s.teams - 1) / s.teams + unit - 1) / unit * unit;
+  return std::min(need, std::max(unit, (int64_t)kSMs * per_sm / unit * unit));
+}
+constexpr int kBackwardThreads = 1024;  // per SM, the most that the workspace provides for
+int backward_most(const Split& s) { return std::max(1, kBackwardThreads / s.block()); }
 
-template <typename TX, typename TZ, int V, int CH>
-void launch_forward(const NormArgs& a, const Split& s, int grid, bool fused, cudaStream_t st) {
-  if (fused)
-    norm_forward_kernel<TX, TZ, V, CH, true><<<grid, s.block, 0, st>>>(a);
-  else if constexpr (sizeof(TX) == sizeof(TZ))
-    norm_forward_kernel<TX, TZ, V, CH, false><<<grid, s.block, 0, st>>>(a);
+// CTAs of a kernel that an SM holds, remembered for the last block and shared-memory size asked for.
+template <typename Kernel>
+int32_t resident(Kernel kernel, std::atomic<uint64_t>& memo, int block, size_t smem, int* per_sm) {
+  const uint64_t key = (uint64_t)block << 40 | (uint64_t)smem << 8, seen = memo.load(std::memory_order_relaxed);
+  if ((seen & ~(uint64_t)255) == key && (seen & 255) != 0) {
+    *per_sm = (int)(seen & 255);
+    return PLSTM_OK;
+  }
+  if (smem > 40 * 1024)
+    PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  PLSTM_TRY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kernel, block, smem));
+  *per_sm = std::max(1, *per_sm);
+  memo.store(key | (uint64_t)*per_sm, std::memory_order_relaxed);
+  return PLSTM_OK;
 }
 
-template <typename TX, typename TZ, int V, int CH>
-void launch_backward(const NormArgs& a, const Split& s, int grid, bool fused, cudaStream_t st) {
-  const size_t smem = s.block > s.tpr ? (size_t)a.cols * 2 * sizeof(float) : 0;
-  if (fused)
-    norm_backward_kernel<TX, TZ, V, CH, true><<<grid, s.block, smem, st>>>(a);
-  else if constexpr (sizeof(TX) == sizeof(TZ))
-    norm_backward_kernel<TX, TZ, V, CH, false><<<grid, s.block, smem, st>>>(a);
+template <bool BACKWARD, typename Kernel>
+int32_t launch(Kernel kernel, std::atomic<uint64_t>& memo, const plstm_norm_desc& d, const NormArgs& a, const Split& s,
+               size_t smem, int* grid, cudaStream_t st) {
+  int per_sm = 0;
+  if (const int32_t rc = resident(kernel, memo, s.block(), smem, &per_sm)) return rc;
+  *grid = (int)(BACKWARD ? backward_ctas(d, s, std::min(per_sm, backward_most(s))) : forward_ctas(d, s, per_sm));
+  kernel<<<*grid, s.block(), smem, st>>>(a);
+  PLSTM_TRY_CUDA(cudaGetLastError());
+  note_launches(1);
+  return PLSTM_OK;
+}
+
+template <typename TX, typename TZ, int CH, bool FUSED, bool WHOLE>
+int32_t launch_kernel(bool backward, const plstm_norm_desc& d, const NormArgs& a, const Split& s, int* grid,
+                      cudaStream_t st) {
+  static std::atomic<uint64_t> memo[2];
+  if (backward)
+    return launch<true>(norm_backward_kernel<TX, TZ, CH, FUSED, WHOLE>, memo[1], d, a, s, backward_smem(d, s), grid, st);
+  return launch<false>(norm_forward_kernel<TX, TZ, CH, FUSED, WHOLE>, memo[0], d, a, s, forward_smem(d), grid, st);
+}
+
+template <typename TX, typename TZ, bool FUSED, bool WHOLE>
+int32_t launch_split(bool backward, const plstm_norm_desc& d, NormArgs& a, int* grid, cudaStream_t st) {
+  const Split s = make_split(d, WHOLE, backward);
+  a.tpr = s.tpr;
+  a.teams = s.teams;
+  if (s.ch == 1) return launch_kernel<TX, TZ, 1, FUSED, WHOLE>(backward, d, a, s, grid, st);
+  if (s.ch == 2) return launch_kernel<TX, TZ, 2, FUSED, WHOLE>(backward, d, a, s, grid, st);
+  return launch_kernel<TX, TZ, 4, FUSED, WHOLE>(backward, d, a, s, grid, st);
 }
 
 template <typename TX, typename TZ>
-void dispatch(bool backward, const NormArgs& a, const Split& s, int grid, bool fused, cudaStream_t st) {
-  constexpr int VF = 16 / sizeof(TX);
-#define PLSTM_NORM_CASE(V, CH)                                              \
-  if (s.v == V && s.ch == CH) {                                             \
-    if (backward)                                                           \
-      launch_backward<TX, TZ, V, CH>(a, s, grid, fused, st);                \
-    else                                                                    \
-      launch_forward<TX, TZ, V, CH>(a, s, grid, fused, st);                 \
-    return;                                                                 \
+int32_t dispatch(bool backward, const plstm_norm_desc& d, NormArgs& a, bool fused, bool whole, int* grid, cudaStream_t st) {
+  if constexpr (sizeof(TX) == sizeof(TZ)) {
+    if (!fused)
+      return whole ? launch_split<TX, TZ, false, true>(backward, d, a, grid, st)
+                   : launch_split<TX, TZ, false, false>(backward, d, a, grid, st);
   }
-  PLSTM_NORM_CASE(VF, 1)
-  PLSTM_NORM_CASE(VF, 2)
-  PLSTM_NORM_CASE(VF, 4)
-  PLSTM_NORM_CASE(1, 1)
-  PLSTM_NORM_CASE(1, 2)
-  PLSTM_NORM_CASE(1, 4)
-  PLSTM_NORM_CASE(1, 16)
-#undef PLSTM_NORM_CASE
+  return whole ? launch_split<TX, TZ, true, true>(backward, d, a, grid, st)
+               : launch_split<TX, TZ, true, false>(backward, d, a, grid, st);
 }
 
-void dispatch_types(bool backward, const plstm_norm_desc& d, const NormArgs& a, const Split& s, int grid, bool fused,
-                    cudaStream_t st) {
+// `grid` receives the CTAs launched.
+int32_t dispatch_types(bool backward, const plstm_norm_desc& d, NormArgs& a, bool fused, bool whole, int* grid,
+                       cudaStream_t st) {
   if (d.x_dtype == PLSTM_F32)
-    dispatch<float, float>(backward, a, s, grid, fused, st);
-  else if (d.x_dtype == PLSTM_F16 && d.z_dtype == PLSTM_F16)
-    dispatch<__half, __half>(backward, a, s, grid, fused, st);
-  else if (d.x_dtype == PLSTM_F16)
-    dispatch<__half, float>(backward, a, s, grid, fused, st);
-  else if (d.z_dtype == PLSTM_BF16)
-    dispatch<__nv_bfloat16, __nv_bfloat16>(backward, a, s, grid, fused, st);
-  else
-    dispatch<__nv_bfloat16, float>(backward, a, s, grid, fused, st);
+    return dispatch<float, float>(backward, d, a, fused, whole, grid, st);
+  if (d.x_dtype == PLSTM_F16 && d.z_dtype == PLSTM_F16)
+    return dispatch<__half, __half>(backward, d, a, fused, whole, grid, st);
+  if (d.x_dtype == PLSTM_F16)
+    return dispatch<__half, float>(backward, d, a, fused, whole, grid, st);
+  if (d.z_dtype == PLSTM_BF16)
+    return dispatch<__nv_bfloat16, __nv_bfloat16>(backward, d, a, fused, whole, grid, st);
+  return dispatch<__nv_bfloat16, float>(backward, d, a, fused, whole, grid, st);
 }
 
 int32_t check_desc(const plstm_norm_desc* d, bool fused) {
@@ -407,9 +652,17 @@ int32_t check_desc(const plstm_norm_desc* d, bool fused) {
   return PLSTM_OK;
 }
 
-// Every row of the tensor starts on a 16-byte boundary.
-bool rows16(const void* p, int64_t stride, int32_t dtype) {
-  return p == nullptr || (aligned16(p) && stride * (int64_t)dtype_size(dtype) % 16 == 0);
+// A chunk at column col of row r lies at r * stride + col with r * cols + col a multiple of 8.
+Mat make_mat(const plstm_norm_desc& d, const void* p, int64_t stride, int32_t dtype) {
+  const int64_t size = (int64_t)dtype_size(dtype);
+  if (d.rows == 1) stride = d.cols;
+  return Mat{p, stride, (d.rows - 1) * stride + d.cols, aligned16(p) && (stride - d.cols) * size % 16 == 0};
+}
+bool all_whole(const plstm_norm_desc& d, std::initializer_list<const Mat*> all) {
+  if (d.cols % 8 != 0) return false;
+  for (const Mat* m : all)
+    if (!m->vec) return false;
+  return true;
 }
 
 }  // namespace
@@ -438,29 +691,21 @@ int32_t plstm_layer_norm_forward(const plstm_norm_desc* d, const plstm_dropout_d
                   "layer norm: a pointer is not aligned to its element");
   DeviceGuard guard;
   if (const int32_t rc = guard.enter(d->device)) return rc;
-  const bool vec = d->cols % (16 / xs) == 0 && rows16(x, d->x_stride, d->x_dtype) && aligned16(y) &&
-                   rows16(residual, d->residual_stride, d->z_dtype) && aligned16(z) && aligned16(weight) &&
-                   aligned16(bias);
-  const Split s = make_split(*d, vec);
   a.rows = d->rows;
   a.cols = d->cols;
-  a.tpr = s.tpr;
   a.eps = d->eps;
-  a.x_stride = d->x_stride;
-  a.res_stride = d->residual_stride;
-  a.x = x;
-  a.residual = residual;
+  a.x = make_mat(*d, x, d->x_stride, d->x_dtype);
+  a.residual = make_mat(*d, residual, d->residual_stride, d->z_dtype);
+  a.z = make_mat(*d, z, d->cols, d->z_dtype);
+  a.y = make_mat(*d, y, d->cols, d->x_dtype);
   a.weight = weight;
   a.bias = bias;
-  a.z = z;
-  a.y = y;
   a.mean = stats;
   a.rstd = stats != nullptr ? stats + d->rows : nullptr;
   a.w_dtype = d->w_dtype;
-  dispatch_types(false, *d, a, s, (int)row_ctas(*d, s, 2048 / s.block), fused, static_cast<cudaStream_t>(stream));
-  PLSTM_TRY_CUDA(cudaGetLastError());
-  note_launches(1);
-  return PLSTM_OK;
+  const bool whole = fused ? all_whole(*d, {&a.x, &a.residual, &a.z, &a.y}) : all_whole(*d, {&a.x, &a.y});
+  int grid = 0;
+  return dispatch_types(false, *d, a, fused, whole, &grid, static_cast<cudaStream_t>(stream));
 }
 
 int32_t plstm_layer_norm_backward_workspace_size(const plstm_norm_desc* d, size_t* bytes) {
@@ -468,8 +713,11 @@ int32_t plstm_layer_norm_backward_workspace_size(const plstm_norm_desc* d, size_
   PLSTM_CHECK_ARG(bytes != nullptr, "bytes is NULL");
   if (const int32_t rc = check_desc(d, true)) return rc;
   // The larger of the two splits that alignment chooses between.
-  const Split s0 = make_split(*d, false), s1 = make_split(*d, true);
-  const int64_t parts = std::max(row_ctas(*d, s0, backward_per_sm(s0)), row_ctas(*d, s1, backward_per_sm(s1)));
+  int64_t parts = 0;
+  for (const bool whole : {false, d->cols % 8 == 0}) {
+    const Split s = make_split(*d, whole, true);
+    parts = std::max(parts, backward_ctas(*d, s, backward_most(s)));
+  }
   *bytes = (size_t)parts * 2 * (size_t)d->cols * sizeof(float);
   return PLSTM_OK;
 }
@@ -509,30 +757,21 @@ int32_t plstm_layer_norm_backward(const plstm_norm_desc* d, const plstm_dropout_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int parts = 0;
   if (d->rows > 0 && (grads || dx != nullptr || dresidual != nullptr)) {
-    const bool vec = d->cols % (16 / xs) == 0 && rows16(dy, d->dy_stride, d->x_dtype) &&
-                     rows16(v, fused ? d->cols : d->x_stride, d->z_dtype) && rows16(dz, d->dz_stride, d->z_dtype) &&
-                     aligned16(dx) && aligned16(dresidual) && aligned16(weight);
-    const Split s = make_split(*d, vec);
-    parts = (int)row_ctas(*d, s, backward_per_sm(s));
     a.rows = d->rows;
     a.cols = d->cols;
-    a.tpr = s.tpr;
-    a.x_stride = d->x_stride;
-    a.dy_stride = d->dy_stride;
-    a.dz_stride = d->dz_stride;
-    a.dy = dy;
-    a.dz = dz;
-    a.v = v;
+    a.dy = make_mat(*d, dy, d->dy_stride, d->x_dtype);
+    a.dz = make_mat(*d, dz, d->dz_stride, d->z_dtype);
+    a.v = make_mat(*d, v, fused ? d->cols : d->x_stride, d->z_dtype);
+    a.dx = make_mat(*d, dx, d->cols, d->x_dtype);
+    a.dres = make_mat(*d, dresidual, d->cols, d->z_dtype);
     a.weight = weight;
-    a.dx = dx;
-    a.dres = dresidual;
     a.mean = const_cast<float*>(stats);
     a.rstd = const_cast<float*>(stats) + d->rows;
     a.partial = grads ? static_cast<float*>(workspace) : nullptr;
     a.w_dtype = d->w_dtype;
-    dispatch_types(true, *d, a, s, parts, fused != 0, st);
-    PLSTM_TRY_CUDA(cudaGetLastError());
-    note_launches(1);
+    if (dz == nullptr) a.dz.vec = 1;
+    const bool whole = all_whole(*d, {&a.dy, &a.v, &a.dx}) && (!fused || all_whole(*d, {&a.dz, &a.dres}));
+    if (const int32_t rc = dispatch_types(true, *d, a, fused != 0, whole, &parts, st)) return rc;
   }
   if (grads) {
     norm_weight_grad_kernel<<<dim3((d->cols + 31) / 32, 2), dim3(32, 32), 0, st>>>(

@@ -86,13 +86,75 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& v) {
   *reinterpret_cast<typename Word<V * sizeof(T)>::type*>(p) = v.word;
 }
 
+// 1 / sqrt(a): the hardware's approximation and one Newton step.
+__device__ __forceinline__ float rsqrt_rn(float a) {
+  const float r = rsqrtf(a);
+  return a > 0.0f && a < INFINITY ? r * fmaf(-0.5f * a * r, r, 1.5f) : r;
+}
+
 inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 inline bool dtype_ok(int32_t dt) { return dt == PLSTM_F32 || dt == PLSTM_F16 || dt == PLSTM_BF16; }
+
+// ---- packed arithmetic -------------------------------------------------------------------------
+// V neighbouring f32 values.  Two of them go through the f32x2 instructions, which do
+// two operations for one issue slot; the special-function unit takes them one by one.
+template <int V>
+struct F;
+template <>
+struct F<1> {
+  float x;
+  __device__ __forceinline__ float get(int) const { return x; }
+  static __device__ __forceinline__ F of(float a) { return {a}; }
+  static __device__ __forceinline__ F of(const float (&a)[1]) { return {a[0]}; }
+};
+template <>
+struct F<2> {
+  uint64_t p;
+  __device__ __forceinline__ float get(int k) const { return __uint_as_float((uint32_t)(k ? p >> 32 : p)); }
+  static __device__ __forceinline__ F of(float lo, float hi) {
+    return {(uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo)};
+  }
+  static __device__ __forceinline__ F of(float a) { return of(a, a); }
+  static __device__ __forceinline__ F of(const float (&a)[2]) { return of(a[0], a[1]); }
+};
+__device__ __forceinline__ F<1> fma(F<1> a, F<1> b, F<1> c) { return {fmaf(a.x, b.x, c.x)}; }
+__device__ __forceinline__ F<1> operator*(F<1> a, F<1> b) { return {a.x * b.x}; }
+__device__ __forceinline__ F<1> operator+(F<1> a, F<1> b) { return {a.x + b.x}; }
+__device__ __forceinline__ F<2> fma(F<2> a, F<2> b, F<2> c) {
+  F<2> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.p) : "l"(a.p), "l"(b.p), "l"(c.p));
+  return r;
+}
+__device__ __forceinline__ F<2> operator*(F<2> a, F<2> b) {
+  F<2> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
+  return r;
+}
+__device__ __forceinline__ F<2> operator+(F<2> a, F<2> b) {
+  F<2> r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
+  return r;
+}
+template <int V, typename Fn>
+__device__ __forceinline__ F<V> each(F<V> a, Fn fn) {
+  float r[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) r[k] = fn(a.get(k));
+  return F<V>::of(r);
+}
+// a * b + 1 and the like with a constant in every lane.
+template <int V>
+__device__ __forceinline__ F<V> fma(F<V> a, F<V> b, float c) { return fma(a, b, F<V>::of(c)); }
+template <int V>
+__device__ __forceinline__ F<V> one_plus(F<V> a) { return a + F<V>::of(1.0f); }
+template <int V>
+__device__ __forceinline__ F<V> one_minus(F<V> a) { return fma(a, F<V>::of(-1.0f), F<V>::of(1.0f)); }
 
 // ---- Philox4x32-10 ------------------------------------------------------------------------
 // Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3" (SC 2011): ten
 // rounds of two 32 x 32 -> 64-bit products and key additions (Weyl sequence) on a 128-bit
 // counter.  One call gives the words of four consecutive elements.
+// `seed` comes as a warp-uniform value (uniform_seed), so the round keys cost no vector operations.
 __device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint64_t seed) {
   uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
   uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
@@ -118,7 +180,13 @@ struct Drop {
   int mode;            // 0: keep everything, 1: draw, 2: drop everything (p = 1)
 };
 
-__device__ __forceinline__ uint64_t drop_seed(const Drop& d) { return d.seed_ptr != nullptr ? *d.seed_ptr : d.seed; }
+// The seed, from the descriptor or from the GPU's memory.  Every lane holds the same value; the
+// reductions tell the compiler so.  All lanes of the warp have to call this.
+__device__ __forceinline__ uint64_t uniform_seed(const Drop& d) {
+  const uint64_t s = d.seed_ptr != nullptr ? *d.seed_ptr : d.seed;
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)s), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(s >> 32));
+  return (uint64_t)hi << 32 | lo;
+}
 
 // x / (1 - p) where the word keeps the element, else 0 (whatever x is).  The explicit
 // rounding keeps the compiler from contracting the product with a later sum, so that the
@@ -126,28 +194,24 @@ __device__ __forceinline__ uint64_t drop_seed(const Drop& d) { return d.seed_ptr
 __device__ __forceinline__ float drop_one(const Drop& d, uint32_t word, float x) {
   return word >= d.threshold ? __fmul_rn(x, d.scale) : 0.0f;
 }
-__device__ __forceinline__ uint32_t word_of(const uint4& w, int k) {
-  return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
-}
 
-// Applies the dropout to the V elements from flattened index e on.  V = 4 or 8 needs e % 4 == 0.
+// Applies the dropout to the V (4 or 8) elements from flattened index e on; e % 4 == 0.
 template <int V>
 __device__ __forceinline__ void drop_vec(const Drop& d, uint64_t seed, int64_t e, float (&x)[V]) {
+  static_assert(V % 4 == 0, "whole Philox blocks");
   if (d.mode == 0) return;
   if (d.mode == 2) {
 #pragma unroll
     for (int k = 0; k < V; ++k) x[k] = 0.0f;
     return;
   }
-  if constexpr (V == 1) {
-    x[0] = drop_one(d, word_of(philox((uint64_t)e >> 2, d.offset, seed), (int)(e & 3)), x[0]);
-  } else {
 #pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const uint4 w = philox(((uint64_t)e >> 2) + q, d.offset, seed);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[4 * q + k] = drop_one(d, word_of(w, k), x[4 * q + k]);
-    }
+  for (int q = 0; q < V / 4; ++q) {
+    const uint4 w = philox(((uint64_t)e >> 2) + q, d.offset, seed);
+    x[4 * q] = drop_one(d, w.x, x[4 * q]);
+    x[4 * q + 1] = drop_one(d, w.y, x[4 * q + 1]);
+    x[4 * q + 2] = drop_one(d, w.z, x[4 * q + 2]);
+    x[4 * q + 3] = drop_one(d, w.w, x[4 * q + 3]);
   }
 }
 

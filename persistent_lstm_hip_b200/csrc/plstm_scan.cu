@@ -50,61 +50,6 @@ struct ScanArgs {
   float* dc0;
 };
 
-// ---- packed arithmetic -------------------------------------------------------------------------
-// V f32 values of neighbouring channels.  Two of them go through the f32x2 instructions, which do
-// two operations for one issue slot; the special-function unit takes them one by one.
-template <int V>
-struct F;
-template <>
-struct F<1> {
-  float x;
-  __device__ __forceinline__ float get(int) const { return x; }
-  static __device__ __forceinline__ F of(float a) { return {a}; }
-  static __device__ __forceinline__ F of(const float (&a)[1]) { return {a[0]}; }
-};
-template <>
-struct F<2> {
-  uint64_t p;
-  __device__ __forceinline__ float get(int k) const { return __uint_as_float((uint32_t)(k ? p >> 32 : p)); }
-  static __device__ __forceinline__ F of(float lo, float hi) {
-    return {(uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo)};
-  }
-  static __device__ __forceinline__ F of(float a) { return of(a, a); }
-  static __device__ __forceinline__ F of(const float (&a)[2]) { return of(a[0], a[1]); }
-};
-__device__ __forceinline__ F<1> fma(F<1> a, F<1> b, F<1> c) { return {fmaf(a.x, b.x, c.x)}; }
-__device__ __forceinline__ F<1> operator*(F<1> a, F<1> b) { return {a.x * b.x}; }
-__device__ __forceinline__ F<1> operator+(F<1> a, F<1> b) { return {a.x + b.x}; }
-__device__ __forceinline__ F<2> fma(F<2> a, F<2> b, F<2> c) {
-  F<2> r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.p) : "l"(a.p), "l"(b.p), "l"(c.p));
-  return r;
-}
-__device__ __forceinline__ F<2> operator*(F<2> a, F<2> b) {
-  F<2> r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
-  return r;
-}
-__device__ __forceinline__ F<2> operator+(F<2> a, F<2> b) {
-  F<2> r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
-  return r;
-}
-template <int V, typename Fn>
-__device__ __forceinline__ F<V> each(F<V> a, Fn fn) {
-  float r[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) r[k] = fn(a.get(k));
-  return F<V>::of(r);
-}
-// a * b + 1 and the like with a constant in every lane.
-template <int V>
-__device__ __forceinline__ F<V> fma(F<V> a, F<V> b, float c) { return fma(a, b, F<V>::of(c)); }
-template <int V>
-__device__ __forceinline__ F<V> one_plus(F<V> a) { return a + F<V>::of(1.0f); }
-template <int V>
-__device__ __forceinline__ F<V> one_minus(F<V> a) { return fma(a, F<V>::of(-1.0f), F<V>::of(1.0f)); }
-
 // One special-function instruction each; results below 2^-126 come out as 0, 1 / inf as 0.
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -319,7 +264,7 @@ struct Exchange {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kMaxThreads) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+__global__ void __launch_bounds__(kMaxThreads, 3) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
   constexpr bool PRECISE = sizeof(T) == 4;
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
@@ -376,7 +321,7 @@ __global__ void __launch_bounds__(kMaxThreads) scan_forward_kernel(const __grid_
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kMaxThreads) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+__global__ void __launch_bounds__(kMaxThreads, 2) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
   constexpr bool PRECISE = sizeof(T) == 4;
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);

@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_forward_k
 // all have one phase (their distance is a multiple of 8), so a thread's columns stay its own and
 // the sums of the weight gradients stay with it: in registers, or (CH = 4) in shared memory.
 template <typename TX, typename TV, int CH, bool FUSED, bool WHOLE>
-__global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(max_block(CH), CH == 1 ? 2 : 1) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr bool REGS = CH < 4;
   __shared__ float scratch[2 * 2 * 32 * (kTeamBlock / 32)];
   extern __shared__ __align__(16) float columns[];
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_
         acc[(c * 4 + k) * tpr] = acc[((CH + c) * 4 + k) * tpr] = F<2>::of(0.0f);
     }
   }
-  // Rows are fetched a turn ahead where the registers hold two (CH = 1).
-  constexpr bool AHEAD = CH == 1;
+  // Rows are fetched a turn ahead where the registers hold two.
+  constexpr bool AHEAD = CH <= 2, KEEP_W = CH == 1;
   Chunk<TX> next_dy[AHEAD ? CH : 1];
   Chunk<TV> next_in[AHEAD ? CH : 1];
   float next_mean = 0.0f, next_rstd = 0.0f;
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_
   w.fill(a.weight, a.w_dtype, cols, 1.0f);
   __syncthreads();
   F<2> ww[4];
-  if (AHEAD && col0 < cols) w.read(col0, ww);
+  if (KEEP_W && col0 < cols) w.read(col0, ww);
   int turn = 0;
   for (int64_t head = at.first; head < a.rows; head += at.step, ++turn) {
     const int64_t row = head + at.within;
@@ -371,8 +371,11 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_
     Chunk<TV> in[CH], dz[FUSED ? CH : 1];
     float mean = 0.0f, rstd = 0.0f;
     if constexpr (AHEAD) {
-      dy[0] = next_dy[0];
-      in[0] = next_in[0];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        dy[c] = next_dy[c];
+        in[c] = next_in[c];
+      }
       mean = next_mean;
       rstd = next_rstd;
       fetch(row + at.step, next_dy, next_in, next_mean, next_rstd);
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_
     for (int c = 0; c < CH; ++c) {
       const int col = col0 + c * tpr * 8;
       if (live && col < cols) {
-        if constexpr (!AHEAD) w.read(col, ww);
+        if constexpr (!KEEP_W) w.read(col, ww);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           // dy is zero outside the row, and so is every sum's term there.
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_backward_
     for (int c = 0; c < CH; ++c) {
       const int col = col0 + c * tpr * 8;
       if (col < cols) {
-        if constexpr (!AHEAD) w.read(col, ww);
+        if constexpr (!KEEP_W) w.read(col, ww);
         float dv[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -535,7 +538,7 @@ Split make_split(const plstm_norm_desc& d, bool whole, bool backward) {
   const bool f32 = d.x_dtype == PLSTM_F32;
   s.ch = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
   if (f32 && chunks <= 513) s.ch = std::min(s.ch, 2);
-  if (backward) s.ch = chunks <= 257 ? 1 : chunks <= 513 ? 2 : 4;
+  if (backward) s.ch = chunks <= 48 ? 1 : chunks <= 513 ? 2 : 4;
   const int threads = (chunks + s.ch - 1) / s.ch;
   if (threads >= 32) {
     s.tpr = (threads + 31) / 32 * 32;

@@ -46,8 +46,12 @@ __global__ void __launch_bounds__(kThreads, 4) dropout_kernel(Drop d, int64_t n,
                                                               const TY* __restrict__ residual, TY* __restrict__ y) {
   const uint64_t seed = uniform_seed(d);
   const int64_t groups = (n + 7) / 8, whole = ALIGNED ? n / 8 : 0;
-  for (int64_t base = blockIdx.x * (int64_t)(kThreads * kUnroll) + threadIdx.x; base < groups;
-       base += (int64_t)gridDim.x * (kThreads * kUnroll)) {
+  for (int64_t first = blockIdx.x * (int64_t)(kThreads * kUnroll); first < groups;
+       first += (int64_t)gridDim.x * (kThreads * kUnroll)) {
+    // `first` and with it the upper word of its Philox block is the CTA's own; its lowest 10 bits are
+    // zero, so the thread's place never carries into that word.
+    const int64_t base = first + threadIdx.x;
+    const uint32_t block = (uint32_t)(2 * first), block_hi = (uint32_t)(2 * first >> 32);
     Eight<TX> in[kUnroll];
     Eight<TY> res[RESIDUAL ? kUnroll : 1];
 #pragma unroll
@@ -65,7 +69,7 @@ __global__ void __launch_bounds__(kThreads, 4) dropout_kernel(Drop d, int64_t n,
       if (g < whole) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = in[u].get(k);
-        drop_vec<8>(d, seed, e, v);
+        drop_eight(d, seed, block + 2 * (u * kThreads + threadIdx.x), block_hi, v);
         if constexpr (RESIDUAL) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(res[u].get(k), v[k]);
@@ -75,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 4) dropout_kernel(Drop d, int64_t n,
       } else if (g < groups) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = e + k < n ? to_f32(x[e + k]) : 0.0f;
-        drop_vec<8>(d, seed, e, v);
+        drop_eight(d, seed, block + 2 * (u * kThreads + threadIdx.x), block_hi, v);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           if (e + k < n) y[e + k] = from_f32<TY>(RESIDUAL ? __fadd_rn(to_f32(residual[e + k]), v[k]) : v[k]);

@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_forward_k
           float f[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) f[k] = x[c].get(k);
-          drop_vec<8>(a.drop, seed, row * cols + col, f);
+          const uint64_t block = (uint64_t)(row * cols + col) >> 2;
+          drop_eight(a.drop, seed, (uint32_t)block, (uint32_t)(block >> 32), f);
 #pragma unroll
           for (int k = 0; k < 8; ++k) f[k] = __fadd_rn(r[c].get(k), f[k]);
           r[c].set(f);  // the norm is of z as stored
@@ -441,7 +442,8 @@ __global__ void __launch_bounds__(max_block(CH), CH == 1 ? 2 : 1) norm_backward_
             out.template store<WHOLE>(a.dres, row, col, cols);
           }
           if (a.dx.p == nullptr) continue;
-          drop_vec<8>(a.drop, seed, row * cols + col, dv);
+          const uint64_t block = (uint64_t)(row * cols + col) >> 2;
+          drop_eight(a.drop, seed, (uint32_t)block, (uint32_t)(block >> 32), dv);
         }
         if (a.dx.p != nullptr) {
           Chunk<TX> out;
@@ -513,14 +515,19 @@ __global__ void __launch_bounds__(max_block(CH), CH == 1 ? 2 : 1) norm_backward_
 }
 
 // dweight / dbias from the CTAs' partial sums [parts][2][cols]: 32 columns per CTA, 32 threads
-// deep over the parts, then a fixed tree.
+// deep over the parts, then a fixed tree.  Launched while the backward still runs
+// (programmatic dependent launch); it waits for it before it reads.
 __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __restrict__ partial, int parts, int cols,
                                                                 void* dweight, void* dbias, int w_dtype) {
   __shared__ float sums[32][33];
   const int which = blockIdx.y, col = blockIdx.x * 32 + threadIdx.x;
+  cudaGridDependencySynchronize();
   float s = 0.0f;
-  if (col < cols)
-    for (int p = threadIdx.y; p < parts; p += 32) s += partial[((int64_t)p * 2 + which) * cols + col];
+  if (col < cols) {
+    const float* from = partial + (int64_t)which * cols + col;
+#pragma unroll 8
+    for (int p = threadIdx.y; p < parts; p += 32) s += from[(int64_t)p * 2 * cols];
+  }
   sums[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   s = sums[threadIdx.x][threadIdx.y];
@@ -777,9 +784,17 @@ int32_t plstm_layer_norm_backward(const plstm_norm_desc* d, const plstm_dropout_
     if (const int32_t rc = dispatch_types(true, *d, a, fused != 0, whole, &parts, st)) return rc;
   }
   if (grads) {
-    norm_weight_grad_kernel<<<dim3((d->cols + 31) / 32, 2), dim3(32, 32), 0, st>>>(
-        static_cast<const float*>(workspace), parts, d->cols, dweight, dbias, d->w_dtype);
-    PLSTM_TRY_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((d->cols + 31) / 32, 2);
+    cfg.blockDim = dim3(32, 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, norm_weight_grad_kernel, static_cast<const float*>(workspace), parts,
+                                      (int)d->cols, dweight, dbias, (int)d->w_dtype));
     note_launches(1);
   }
   return PLSTM_OK;

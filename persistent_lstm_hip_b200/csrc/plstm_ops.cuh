@@ -109,30 +109,37 @@ struct F<1> {
 };
 template <>
 struct F<2> {
-  uint64_t p;
-  __device__ __forceinline__ float get(int k) const { return __uint_as_float((uint32_t)(k ? p >> 32 : p)); }
-  static __device__ __forceinline__ F of(float lo, float hi) {
-    return {(uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo)};
-  }
-  static __device__ __forceinline__ F of(float a) { return of(a, a); }
-  static __device__ __forceinline__ F of(const float (&a)[2]) { return of(a[0], a[1]); }
+  float x, y;
+  __device__ __forceinline__ float get(int k) const { return k ? y : x; }
+  static __device__ __forceinline__ F of(float lo, float hi) { return {lo, hi}; }
+  static __device__ __forceinline__ F of(float a) { return {a, a}; }
+  static __device__ __forceinline__ F of(const float (&a)[2]) { return {a[0], a[1]}; }
 };
 __device__ __forceinline__ F<1> fma(F<1> a, F<1> b, F<1> c) { return {fmaf(a.x, b.x, c.x)}; }
 __device__ __forceinline__ F<1> operator*(F<1> a, F<1> b) { return {a.x * b.x}; }
 __device__ __forceinline__ F<1> operator+(F<1> a, F<1> b) { return {a.x + b.x}; }
 __device__ __forceinline__ F<2> fma(F<2> a, F<2> b, F<2> c) {
   F<2> r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.p) : "l"(a.p), "l"(b.p), "l"(c.p));
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+      "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
 __device__ __forceinline__ F<2> operator*(F<2> a, F<2> b) {
   F<2> r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\n"
+      "mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 __device__ __forceinline__ F<2> operator+(F<2> a, F<2> b) {
   F<2> r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.p) : "l"(a.p), "l"(b.p));
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\n"
+      "mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 template <int V, typename Fn>

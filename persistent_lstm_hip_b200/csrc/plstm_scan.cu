@@ -20,6 +20,7 @@
 // time.  c is rebuilt from the state that the forward kept for every segment.
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <initializer_list>
 
 #include "plstm_ops.cuh"
 
@@ -30,8 +31,8 @@ namespace ops {
 namespace {
 
 constexpr int kSeg = PLSTM_SCAN_SEGMENT;
-constexpr int kMaxThreads = 256;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxThreads = 128;
+constexpr int kMaxCluster = 16;
 
 struct ScanArgs {
   int B, T, H;
@@ -98,9 +99,9 @@ template <bool PRECISE, int V>
 __device__ __forceinline__ F<V> sigmoid_f(F<V> x) {
   return each(one_plus(exp_of<PRECISE>(x, -1.0f)), rcp);
 }
-// tanh(x) = num / den.  From 0.3 on (1 - e^-2x) / (1 + e^-2x), of x >= -9.1, where tanh rounds to
-// -1 and the exponential is still small enough to be multiplied with another; below 0.3, where
-// the difference would cancel, the odd series to x^9 (the next term is 4e-8 of the value).
+// tanh(x) = num / den with den = 1 + e^-2x, of x >= -9.1, where tanh rounds to -1 and the exponential
+// is still small enough to be multiplied with another.  num is 1 - e^-2x from 0.3 on; below, where
+// that difference would cancel, den times the odd series to x^9 (the next term is 4e-8 of the value).
 template <bool PRECISE, int V>
 __device__ __forceinline__ void tanh_parts(F<V> x, F<V>& num, F<V>& den) {
   const F<V> e = exp_of<PRECISE>(each(x, [](float v) { return max_nan(v, -9.1f); }), -2.0f);
@@ -109,16 +110,12 @@ __device__ __forceinline__ void tanh_parts(F<V> x, F<V>& num, F<V>& den) {
   p = fma(s, p, 2.0f / 15);
   p = fma(s, p, -1.0f / 3);
   p = fma(x * s, p, x);
-  const F<V> n = one_minus(e), d = one_plus(e);
-  float rn[V], rd[V];
+  den = one_plus(e);
+  const F<V> n = one_minus(e), q = p * den;
+  float r[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const bool small = fabsf(x.get(k)) < 0.3f;
-    rn[k] = small ? p.get(k) : n.get(k);
-    rd[k] = small ? 1.0f : d.get(k);
-  }
-  num = F<V>::of(rn);
-  den = F<V>::of(rd);
+  for (int k = 0; k < V; ++k) r[k] = fabsf(x.get(k)) < 0.3f ? q.get(k) : n.get(k);
+  num = F<V>::of(r);
 }
 template <bool PRECISE, int V>
 __device__ __forceinline__ F<V> tanh_f(F<V> x) {
@@ -134,9 +131,68 @@ __device__ __forceinline__ F<V> sigmoid_tanh(F<V> a, F<V> x) {
   return num * each(one_plus(exp_of<PRECISE>(a, -1.0f)) * den, rcp);
 }
 
+// What a thread holds of a step: V channels as packs of two values, or of one.
 template <int V>
-struct alignas(8 * V) Run {  // the action c -> a c + b of a run of steps
-  F<V> a, b;
+struct Lanes {
+  static constexpr int W = V == 1 ? 1 : 2, N = V / W;
+  F<W> p[N];
+  static __device__ __forceinline__ Lanes of(float a) {
+    Lanes r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.p[i] = F<W>::of(a);
+    return r;
+  }
+  __device__ __forceinline__ float get(int k) const { return p[k / W].get(k % W); }
+};
+template <int V, typename Fn>
+__device__ __forceinline__ Lanes<V> map(Fn fn, const Lanes<V>& a) {
+  Lanes<V> r;
+#pragma unroll
+  for (int i = 0; i < Lanes<V>::N; ++i) r.p[i] = fn(a.p[i]);
+  return r;
+}
+template <int V, typename Fn>
+__device__ __forceinline__ Lanes<V> map(Fn fn, const Lanes<V>& a, const Lanes<V>& b) {
+  Lanes<V> r;
+#pragma unroll
+  for (int i = 0; i < Lanes<V>::N; ++i) r.p[i] = fn(a.p[i], b.p[i]);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Lanes<V> fma(const Lanes<V>& a, const Lanes<V>& b, const Lanes<V>& c) {
+  Lanes<V> r;
+#pragma unroll
+  for (int i = 0; i < Lanes<V>::N; ++i) r.p[i] = fma(a.p[i], b.p[i], c.p[i]);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Lanes<V> operator*(const Lanes<V>& a, const Lanes<V>& b) {
+  return map([](auto x, auto y) { return x * y; }, a, b);
+}
+template <int V>
+__device__ __forceinline__ Lanes<V> operator+(const Lanes<V>& a, const Lanes<V>& b) {
+  return map([](auto x, auto y) { return x + y; }, a, b);
+}
+template <int V>
+__device__ __forceinline__ Lanes<V> one_less(const Lanes<V>& a) {
+  return map([](auto x) { return one_minus(x); }, a);
+}
+template <bool PRECISE, int V>
+__device__ __forceinline__ Lanes<V> sigmoids(const Lanes<V>& a) {
+  return map([](auto x) { return sigmoid_f<PRECISE>(x); }, a);
+}
+template <bool PRECISE, int V>
+__device__ __forceinline__ Lanes<V> tanhs(const Lanes<V>& a) {
+  return map([](auto x) { return tanh_f<PRECISE>(x); }, a);
+}
+template <bool PRECISE, int V>
+__device__ __forceinline__ Lanes<V> sigmoid_tanhs(const Lanes<V>& a, const Lanes<V>& b) {
+  return map([](auto x, auto y) { return sigmoid_tanh<PRECISE>(x, y); }, a, b);
+}
+
+template <int V>
+struct alignas(V == 1 ? 8 : 16) Run {  // the action c -> a c + b of a run of steps
+  Lanes<V> a, b;
 };
 
 // Reads V elements; those past the length are given as the step that changes nothing.
@@ -156,37 +212,43 @@ __device__ __forceinline__ Vec<T, V> constant_vec(uint32_t bits) {
   return v;
 }
 template <typename T, int V>
-__device__ __forceinline__ F<V> widen(const Vec<T, V>& v) {
-  float r[V];
+__device__ __forceinline__ Lanes<V> widen(const Vec<T, V>& v) {
+  Lanes<V> r;
 #pragma unroll
-  for (int k = 0; k < V; ++k) r[k] = v.get(k);
-  return F<V>::of(r);
+  for (int i = 0; i < Lanes<V>::N; ++i) {
+    if constexpr (V == 1)
+      r.p[i] = F<1>::of(v.get(0));
+    else
+      r.p[i] = F<2>::of(v.get(2 * i), v.get(2 * i + 1));
+  }
+  return r;
 }
-// Rounds to T; zero where the step is past the length.
 template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> narrow(F<V> f, bool in) {
+__device__ __forceinline__ Vec<T, V> narrow(const Lanes<V>& f) {
   float r[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) r[k] = f.get(k);
   Vec<T, V> v;
   v.set(r);
-  if constexpr (V * sizeof(T) == 2) {
-    if (!in) v.word = 0;
-  } else {
-#pragma unroll
-    for (int k = 0; k < (int)(V * sizeof(T) / 4); ++k) v.w[k] = in ? v.w[k] : 0u;
-  }
   return v;
 }
 template <int V>
-__device__ __forceinline__ F<V> load_state(const float* p, int64_t at, bool live) {
+__device__ __forceinline__ Lanes<V> load_state(const float* p, int64_t at, bool live) {
   float r[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) r[k] = live && p != nullptr ? p[at + k] : 0.0f;
-  return F<V>::of(r);
+  Lanes<V> f;
+#pragma unroll
+  for (int i = 0; i < Lanes<V>::N; ++i) {
+    if constexpr (V == 1)
+      f.p[i] = F<1>::of(r[0]);
+    else
+      f.p[i] = F<2>::of(r[2 * i], r[2 * i + 1]);
+  }
+  return f;
 }
 template <int V>
-__device__ __forceinline__ void store_state(float* p, int64_t at, F<V> f) {
+__device__ __forceinline__ void store_state(float* p, int64_t at, const Lanes<V>& f) {
 #pragma unroll
   for (int k = 0; k < V; ++k) p[at + k] = f.get(k);
 }
@@ -218,53 +280,80 @@ struct Exchange {
   Run<V>* segs;   // [2][seg][cl]
   Run<V>* ranks;  // [2][kMaxCluster][cl]
 
-  __device__ __forceinline__ F<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
-                                             F<V>& carry) const {
+  __device__ __forceinline__ Lanes<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
+                                                 Lanes<V>& carry) const {
     const int parity = turn & 1;
-    Run<V>* mine = segs + parity * p.seg * p.cl;
+    Run<V>* const mine = segs + parity * p.seg * p.cl + at.cl;
     const int order = REVERSE ? p.seg - 1 - at.seg : at.seg;
-    F<V> state = carry;
+    Lanes<V> state = carry;
     if (at.ranks == 1) {
       if (p.seg == 1) {
         carry = fma(own.a, carry, own.b);
         return state;
       }
-      mine[order * p.cl + at.cl] = own;
+      mine[order * p.cl] = own;
       __syncthreads();
-      for (int s = 0; s < p.seg; ++s) {
-        if (s == order) state = carry;
-        const Run<V> r = mine[s * p.cl + at.cl];
-        carry = fma(r.a, carry, r.b);
-      }
+      int s = 0;
+#pragma unroll 4
+      for (; s < order; ++s) carry = fma(mine[s * p.cl].a, carry, mine[s * p.cl].b);
+      state = carry;
+#pragma unroll 4
+      for (; s < p.seg; ++s) carry = fma(mine[s * p.cl].a, carry, mine[s * p.cl].b);
       return state;
     }
-    mine[order * p.cl + at.cl] = own;
+    mine[order * p.cl] = own;
     __syncthreads();
     // The run of the CTA's segments before this thread's, and of all of them.
-    Run<V> all{F<V>::of(1.0f), F<V>::of(0.0f)}, pre = all;
-    for (int s = 0; s < p.seg; ++s) {
-      if (s == order) pre = all;
-      const Run<V> r = mine[s * p.cl + at.cl];
+    Run<V> all{Lanes<V>::of(1.0f), Lanes<V>::of(0.0f)};
+    const auto fold = [&](const Run<V>& r) {
       all.b = fma(r.a, all.b, r.b);
       all.a = r.a * all.a;
-    }
+    };
+    int s = 0;
+#pragma unroll 4
+    for (; s < order; ++s) fold(mine[s * p.cl]);
+    const Run<V> pre = all;
+#pragma unroll 4
+    for (; s < p.seg; ++s) fold(mine[s * p.cl]);
     cg::cluster_group cluster = cg::this_cluster();
-    Run<V>* slots = ranks + parity * kMaxCluster * p.cl;
+    Run<V>* const slots = ranks + parity * kMaxCluster * p.cl + at.cl;
     const int rank_order = REVERSE ? at.ranks - 1 - at.rank : at.rank;
     for (int r = at.seg; r < at.ranks; r += p.seg)  // the segments share the remote stores
-      cluster.map_shared_rank(slots, r)[rank_order * p.cl + at.cl] = all;
+      cluster.map_shared_rank(slots, r)[rank_order * p.cl] = all;
     cluster.sync();
-    for (int r = 0; r < at.ranks; ++r) {
-      if (r == rank_order) state = carry;
-      const Run<V> q = slots[r * p.cl + at.cl];
-      carry = fma(q.a, carry, q.b);
-    }
+    int r = 0;
+    for (; r < rank_order; ++r) carry = fma(slots[r * p.cl].a, carry, slots[r * p.cl].b);
+    state = carry;
+    for (; r < at.ranks; ++r) carry = fma(slots[r * p.cl].a, carry, slots[r * p.cl].b);
     return fma(pre.a, state, pre.b);
   }
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kMaxThreads, 3) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+// K consecutive steps of V channels of NQ rows of gates (and, with dh, the gradient of h).  Steps from
+// the length on are given as the step that changes nothing: an infinite forget gate over zeros.
+template <typename T, int V, int K>
+__device__ __forceinline__ void load_steps(const T* from, int64_t stride, int H, bool live, int left,
+                                           Vec<T, V> (&raw)[4][K]) {
+  if (live && left >= K) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) raw[q][j] = load_vec<T, V>(from + j * stride + (int64_t)q * H);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        raw[q][j] = live && j < left ? load_vec<T, V>(from + j * stride + (int64_t)q * H)
+                                     : constant_vec<T, V>(q == 1 ? infinity_bits<T>() : 0);
+    }
+  }
+}
+
+// K: steps of a segment; the state entering every kSeg-th step is kept for the backward.
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
   constexpr bool PRECISE = sizeof(T) == 4;
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
@@ -272,46 +361,51 @@ __global__ void __launch_bounds__(kMaxThreads, 3) scan_forward_kernel(const __gr
                                     reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
   // Distributed shared memory may be written once every CTA of the cluster has started.
   if (cluster > 1) cg::this_cluster().sync();
-  const int tile = kSeg * p.seg * cluster;
+  const int tile = K * p.seg * cluster;
   const int turns = (at.len + tile - 1) / tile;
-  const int segments = (p.T + kSeg - 1) / kSeg;
+  const int kept = (p.T + kSeg - 1) / kSeg;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   T* h = static_cast<T*>(p.h) + at.b * p.h_sb + at.ch;
   const int64_t state_at = (int64_t)at.b * p.H + at.ch;
-  F<V> carry = load_state<V>(p.c0, state_at, at.live);
+  Lanes<V> carry = load_state<V>(p.c0, state_at, at.live);
+  const int mine = (at.rank * p.seg + at.seg) * K;
+  Vec<T, V> raw[4][K];
+  load_steps<T, V, K>(gates + mine * p.g_st, p.g_st, p.H, at.live, at.len - mine, raw);
   for (int turn = 0; turn < turns; ++turn) {
-    const int t0 = turn * tile + (at.rank * p.seg + at.seg) * kSeg;
-    Vec<T, V> raw[4][kSeg];
-    const T* from = gates + t0 * p.g_st;
+    const int t0 = turn * tile + mine;
+    Lanes<V> f[K], u[K];
+    Run<V> own{Lanes<V>::of(1.0f), Lanes<V>::of(0.0f)};
 #pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      const bool in = at.live && t0 + j < at.len;
+    for (int j = 0; j < K; ++j) {
+      f[j] = sigmoids<PRECISE>(widen<T, V>(raw[1][j]));
+      u[j] = sigmoid_tanhs<PRECISE>(widen<T, V>(raw[0][j]), widen<T, V>(raw[2][j]));
+      own.b = j == 0 ? u[0] : fma(f[j], own.b, u[j]);
+      own.a = j == 0 ? f[0] : own.a * f[j];
+    }
+    // The next turn's gates are on their way during the exchange and the second pass.
+    Vec<T, V> out_gate[K];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        // f = 1, u = 0: an infinite forget gate over a zero candidate.
-        raw[q][j] = in ? load_vec<T, V>(from + (int64_t)q * p.H) : constant_vec<T, V>(q == 1 ? infinity_bits<T>() : 0);
+    for (int j = 0; j < K; ++j) out_gate[j] = raw[3][j];
+    if (turn + 1 < turns)
+      load_steps<T, V, K>(gates + (t0 + tile) * p.g_st, p.g_st, p.H, at.live, at.len - t0 - tile, raw);
+    Lanes<V> c = exchange(p, at, turn, own, carry);
+    if (!at.live) continue;
+    if (p.ckpt != nullptr && t0 < at.len && (K % kSeg == 0 || t0 % kSeg == 0))
+      store_state<V>(p.ckpt, ((int64_t)at.b * kept + t0 / kSeg) * p.H + at.ch, c);
+    T* const to = h + t0 * p.h_st;
+    if (t0 + K <= at.len) {
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        c = fma(f[j], c, u[j]);
+        store_vec<T, V>(to + j * p.h_st, narrow<T, V>(sigmoid_tanhs<PRECISE>(widen<T, V>(out_gate[j]), c)));
       }
-      from += p.g_st;
-    }
-    F<V> f[kSeg], u[kSeg];
-    Run<V> own{F<V>::of(1.0f), F<V>::of(0.0f)};
+    } else {
 #pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      f[j] = sigmoid_f<PRECISE>(widen(raw[1][j]));
-      u[j] = sigmoid_tanh<PRECISE>(widen(raw[0][j]), widen(raw[2][j]));
-      own.b = fma(f[j], own.b, u[j]);
-      own.a = own.a * f[j];
-    }
-    F<V> c = exchange(p, at, turn, own, carry);
-    if (at.live && p.ckpt != nullptr && t0 < at.len)
-      store_state<V>(p.ckpt, ((int64_t)at.b * segments + t0 / kSeg) * p.H + at.ch, c);
-    T* to = h + t0 * p.h_st;
-#pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      c = fma(f[j], c, u[j]);
-      const Vec<T, V> out = narrow<T, V>(sigmoid_tanh<PRECISE>(widen(raw[3][j]), c), t0 + j < at.len);
-      if (at.live && t0 + j < p.T) store_vec<T, V>(to, out);
-      to += p.h_st;
+      for (int j = 0; j < K; ++j) {
+        c = fma(f[j], c, u[j]);
+        const Vec<T, V> out = narrow<T, V>(sigmoid_tanhs<PRECISE>(widen<T, V>(out_gate[j]), c));
+        if (t0 + j < p.T) store_vec<T, V>(to + j * p.h_st, t0 + j < at.len ? out : constant_vec<T, V>(0));
+      }
     }
   }
   if (!at.live) return;
@@ -321,76 +415,85 @@ __global__ void __launch_bounds__(kMaxThreads, 3) scan_forward_kernel(const __gr
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kMaxThreads, 2) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+__global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
   constexpr bool PRECISE = sizeof(T) == 4;
+  constexpr int K = kSeg;
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
   const Exchange<V, true> exchange{reinterpret_cast<Run<V>*>(smem),
                                    reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
   if (cluster > 1) cg::this_cluster().sync();
-  const int tile = kSeg * p.seg * cluster;
+  const int tile = K * p.seg * cluster;
   const int turns = (at.len + tile - 1) / tile;
-  const int segments = (p.T + kSeg - 1) / kSeg;
+  const int kept = (p.T + K - 1) / K;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   const T* dh = p.dh != nullptr ? static_cast<const T*>(p.dh) + at.b * p.h_sb + at.ch : nullptr;
   T* dg = static_cast<T*>(p.dgates) + at.b * p.d_sb + at.ch;
   const int64_t state_at = (int64_t)at.b * p.H + at.ch;
-  F<V> carry = load_state<V>(p.dc_n, state_at, at.live);
+  Lanes<V> carry = load_state<V>(p.dc_n, state_at, at.live);
   for (int turn = 0; turn < turns; ++turn) {
-    const int t0 = (turns - 1 - turn) * tile + (at.rank * p.seg + at.seg) * kSeg;
-    Vec<T, V> raw[4][kSeg], rdh[kSeg];
-    const T* from = gates + t0 * p.g_st;
-    const T* dfrom = dh + t0 * p.h_st;
+    const int t0 = (turns - 1 - turn) * tile + (at.rank * p.seg + at.seg) * K;
+    const int left = at.len - t0;
+    const bool whole = left >= K;
+    Vec<T, V> raw[4][K], rdh[K];
+    load_steps<T, V, K>(gates + t0 * p.g_st, p.g_st, p.H, at.live, left, raw);
 #pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      const bool in = at.live && t0 + j < at.len;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        raw[q][j] = in ? load_vec<T, V>(from + (int64_t)q * p.H) : constant_vec<T, V>(q == 1 ? infinity_bits<T>() : 0);
-      }
-      rdh[j] = in && dh != nullptr ? load_vec<T, V>(dfrom) : constant_vec<T, V>(0);
-      from += p.g_st;
-      dfrom += p.h_st;
-    }
-    F<V> c = load_state<V>(p.ckpt, ((int64_t)at.b * segments + t0 / kSeg) * p.H + at.ch, at.live && t0 < at.len);
+    for (int j = 0; j < K; ++j)
+      rdh[j] = at.live && j < left && dh != nullptr ? load_vec<T, V>(dh + (t0 + j) * p.h_st) : constant_vec<T, V>(0);
+    Lanes<V> c = load_state<V>(p.ckpt, ((int64_t)at.b * kept + t0 / K) * p.H + at.ch, at.live && left > 0);
     // Per step: f, e and what dc is multiplied with in the gradients of i, f and g.
-    F<V> f[kSeg], e[kSeg], wi[kSeg], wf[kSeg], wg[kSeg];
-    T* to = dg + t0 * p.d_st;
+    Lanes<V> f[K], e[K], wi[K], wf[K], wg[K];
+    T* const to = dg + t0 * p.d_st;
 #pragma unroll
-    for (int j = 0; j < kSeg; ++j) {
-      const F<V> si = sigmoid_f<PRECISE>(widen(raw[0][j])), sf = sigmoid_f<PRECISE>(widen(raw[1][j]));
-      const F<V> g = tanh_f<PRECISE>(widen(raw[2][j])), so = sigmoid_f<PRECISE>(widen(raw[3][j]));
-      const F<V> d = widen(rdh[j]);
+    for (int j = 0; j < K; ++j) {
+      const Lanes<V> si = sigmoids<PRECISE>(widen<T, V>(raw[0][j])), sf = sigmoids<PRECISE>(widen<T, V>(raw[1][j]));
+      const Lanes<V> g = tanhs<PRECISE>(widen<T, V>(raw[2][j])), so = sigmoids<PRECISE>(widen<T, V>(raw[3][j]));
       f[j] = sf;
-      wf[j] = c * (sf * one_minus(sf));
-      wi[j] = g * (si * one_minus(si));
-      wg[j] = si * one_minus(g * g);
+      wf[j] = c * (sf * one_less(sf));
+      wi[j] = g * (si * one_less(si));
+      wg[j] = si * one_less(g * g);
       c = fma(sf, c, si * g);
-      const F<V> tc = tanh_f<PRECISE>(c), dso = d * so;
-      e[j] = t0 + j < at.len ? dso * one_minus(tc * tc) : F<V>::of(0.0f);
-      const Vec<T, V> d_o = narrow<T, V>(dso * tc * one_minus(so), t0 + j < at.len);
-      if (at.live && t0 + j < p.T) store_vec<T, V>(to + 3 * (int64_t)p.H, d_o);
-      to += p.d_st;
+      const Lanes<V> tc = tanhs<PRECISE>(c), dso = widen<T, V>(rdh[j]) * so;
+      e[j] = dso * one_less(tc * tc);
+      const Vec<T, V> d_o = narrow<T, V>(dso * tc * one_less(so));
+      if (whole) {
+        if (at.live) store_vec<T, V>(to + j * p.d_st + 3 * (int64_t)p.H, d_o);
+      } else {
+        if (j >= left) e[j] = Lanes<V>::of(0.0f);
+        if (at.live && t0 + j < p.T)
+          store_vec<T, V>(to + j * p.d_st + 3 * (int64_t)p.H, j < left ? d_o : constant_vec<T, V>(0));
+      }
     }
-    Run<V> own{F<V>::of(1.0f), F<V>::of(0.0f)};
+    Run<V> own{f[K - 1], f[K - 1] * e[K - 1]};
 #pragma unroll
-    for (int j = kSeg - 1; j >= 0; --j) {
+    for (int j = K - 2; j >= 0; --j) {
       own.b = f[j] * (e[j] + own.b);
       own.a = own.a * f[j];
     }
-    F<V> G = exchange(p, at, turn, own, carry);
+    Lanes<V> G = exchange(p, at, turn, own, carry);
+    if (!at.live) continue;
+    if (whole) {
 #pragma unroll
-    for (int j = kSeg - 1; j >= 0; --j) {
-      to -= p.d_st;
-      const bool in = t0 + j < at.len;
-      const F<V> dc = e[j] + G;
-      G = f[j] * dc;
-      const Vec<T, V> di = narrow<T, V>(dc * wi[j], in), df = narrow<T, V>(dc * wf[j], in),
-                      dgg = narrow<T, V>(dc * wg[j], in);
-      if (at.live && t0 + j < p.T) {
-        store_vec<T, V>(to, di);
-        store_vec<T, V>(to + p.H, df);
-        store_vec<T, V>(to + 2 * (int64_t)p.H, dgg);
+      for (int j = K - 1; j >= 0; --j) {
+        const Lanes<V> dc = e[j] + G;
+        G = f[j] * dc;
+        T* const at_j = to + j * p.d_st;
+        store_vec<T, V>(at_j, narrow<T, V>(dc * wi[j]));
+        store_vec<T, V>(at_j + p.H, narrow<T, V>(dc * wf[j]));
+        store_vec<T, V>(at_j + 2 * (int64_t)p.H, narrow<T, V>(dc * wg[j]));
+      }
+    } else {
+#pragma unroll
+      for (int j = K - 1; j >= 0; --j) {
+        const Lanes<V> dc = e[j] + G;
+        G = f[j] * dc;
+        const Vec<T, V> none = constant_vec<T, V>(0);
+        T* const at_j = to + j * p.d_st;
+        if (t0 + j < p.T) {
+          store_vec<T, V>(at_j, j < left ? narrow<T, V>(dc * wi[j]) : none);
+          store_vec<T, V>(at_j + p.H, j < left ? narrow<T, V>(dc * wf[j]) : none);
+          store_vec<T, V>(at_j + 2 * (int64_t)p.H, j < left ? narrow<T, V>(dc * wg[j]) : none);
+        }
       }
     }
   }
@@ -409,13 +512,13 @@ struct Plan {
   int cl, seg, cluster, ch_blocks;
 };
 
-Plan make_plan(int B, int T, int H, int V) {
+Plan make_plan(int B, int T, int H, int V, int K) {
   Plan p;
   const int lanes = (H + V - 1) / V;
   p.cl = 1;
   while (p.cl < 32 && p.cl < lanes) p.cl *= 2;
   p.ch_blocks = (lanes + p.cl - 1) / p.cl;
-  const int segments = std::max(1, (T + kSeg - 1) / kSeg);
+  const int segments = std::max(1, (T + K - 1) / K);
   p.seg = 1;
   while (p.seg * p.cl < kMaxThreads && p.seg < segments) p.seg *= 2;
   p.cluster = 1;
@@ -424,9 +527,9 @@ Plan make_plan(int B, int T, int H, int V) {
   return p;
 }
 
-template <typename T, int V>
+template <typename T, int V, int K>
 int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
-  const Plan plan = make_plan(a.B, a.T, a.H, V);
+  const Plan plan = make_plan(a.B, a.T, a.H, V, K);
   a.cl = plan.cl;
   a.seg = plan.seg;
   a.ch_blocks = plan.ch_blocks;
@@ -446,23 +549,42 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (backward)
-    PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, scan_backward_kernel<T, V>, a, plan.cluster));
-  else
-    PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, scan_forward_kernel<T, V>, a, plan.cluster));
-  note_launches(1);
-  return PLSTM_OK;
+  const auto go = [&](auto kernel) -> int32_t {
+    if (plan.cluster > 8)  // beyond the portable size: has to be allowed for the kernel
+      PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan.cluster));
+    note_launches(1);
+    return PLSTM_OK;
+  };
+  if constexpr (K == kSeg) {
+    if (backward) return go(scan_backward_kernel<T, V>);
+  }
+  return go(scan_forward_kernel<T, V, K>);
 }
 
-// Two channels per thread where every access is aligned to the pair, else one.
+// Every access of V channels is aligned to V elements.
+bool aligned_lanes(int dtype, const ScanArgs& a, int V) {
+  const size_t bytes = V * dtype_size(dtype);
+  for (const int64_t s : {(int64_t)a.H, a.g_sb, a.g_st, a.h_sb, a.h_st, a.d_sb, a.d_st})
+    if (s % V != 0) return false;
+  return aligned_to(a.gates, bytes) && aligned_to(a.h, bytes) && aligned_to(a.dh, bytes) && aligned_to(a.dgates, bytes);
+}
+
+template <typename T>
+int32_t dispatch_type(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    // Four channels halve the loads, stores and addresses of an element; four steps then fill the
+    // registers that eight do with two channels.
+    if (!backward && aligned_lanes(dtype, a, 4)) return launch<T, 4, 4>(false, a, s);
+  }
+  if (aligned_lanes(dtype, a, 2)) return launch<T, 2, kSeg>(backward, a, s);
+  return launch<T, 1, kSeg>(backward, a, s);
+}
+
 int32_t dispatch(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
-  const size_t pair = 2 * dtype_size(dtype);
-  const bool even = a.H % 2 == 0 && a.g_sb % 2 == 0 && a.g_st % 2 == 0 && a.h_sb % 2 == 0 && a.h_st % 2 == 0 &&
-                    a.d_sb % 2 == 0 && a.d_st % 2 == 0 && aligned_to(a.gates, pair) && aligned_to(a.h, pair) &&
-                    aligned_to(a.dh, pair) && aligned_to(a.dgates, pair);
-  if (dtype == PLSTM_F32) return even ? launch<float, 2>(backward, a, s) : launch<float, 1>(backward, a, s);
-  if (dtype == PLSTM_F16) return even ? launch<__half, 2>(backward, a, s) : launch<__half, 1>(backward, a, s);
-  return even ? launch<__nv_bfloat16, 2>(backward, a, s) : launch<__nv_bfloat16, 1>(backward, a, s);
+  if (dtype == PLSTM_F32) return dispatch_type<float>(backward, dtype, a, s);
+  if (dtype == PLSTM_F16) return dispatch_type<__half>(backward, dtype, a, s);
+  return dispatch_type<__nv_bfloat16>(backward, dtype, a, s);
 }
 
 int32_t check_desc(const plstm_scan_desc* d) {

@@ -33,11 +33,14 @@ namespace {
 constexpr int kSeg = PLSTM_SCAN_SEGMENT;
 constexpr int kMaxThreads = 128;
 constexpr int kMaxCluster = 16;
+constexpr int kWanted = 384;  // CTAs of 128 threads that fill the GPU: 2.6 on an SM
+constexpr int kAlone = 16 * kSMs;  // warps that do
 
 struct ScanArgs {
   int B, T, H;
-  int cl, seg;        // channel lanes and time segments of a CTA (cl * seg threads)
+  int cl, seg, groups; // channel lanes, time segments and channel groups of a CTA (their product: threads)
   int ch_blocks;      // CTAs (or clusters) along the channels of a row
+  int stage_at;       // where the staged gates begin in shared memory
   int64_t g_sb, g_st, h_sb, h_st, d_sb, d_st;
   const void* gates;
   const int32_t* lengths;
@@ -131,68 +134,9 @@ __device__ __forceinline__ F<V> sigmoid_tanh(F<V> a, F<V> x) {
   return num * each(one_plus(exp_of<PRECISE>(a, -1.0f)) * den, rcp);
 }
 
-// What a thread holds of a step: V channels as packs of two values, or of one.
 template <int V>
-struct Lanes {
-  static constexpr int W = V == 1 ? 1 : 2, N = V / W;
-  F<W> p[N];
-  static __device__ __forceinline__ Lanes of(float a) {
-    Lanes r;
-#pragma unroll
-    for (int i = 0; i < N; ++i) r.p[i] = F<W>::of(a);
-    return r;
-  }
-  __device__ __forceinline__ float get(int k) const { return p[k / W].get(k % W); }
-};
-template <int V, typename Fn>
-__device__ __forceinline__ Lanes<V> map(Fn fn, const Lanes<V>& a) {
-  Lanes<V> r;
-#pragma unroll
-  for (int i = 0; i < Lanes<V>::N; ++i) r.p[i] = fn(a.p[i]);
-  return r;
-}
-template <int V, typename Fn>
-__device__ __forceinline__ Lanes<V> map(Fn fn, const Lanes<V>& a, const Lanes<V>& b) {
-  Lanes<V> r;
-#pragma unroll
-  for (int i = 0; i < Lanes<V>::N; ++i) r.p[i] = fn(a.p[i], b.p[i]);
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Lanes<V> fma(const Lanes<V>& a, const Lanes<V>& b, const Lanes<V>& c) {
-  Lanes<V> r;
-#pragma unroll
-  for (int i = 0; i < Lanes<V>::N; ++i) r.p[i] = fma(a.p[i], b.p[i], c.p[i]);
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Lanes<V> operator*(const Lanes<V>& a, const Lanes<V>& b) {
-  return map([](auto x, auto y) { return x * y; }, a, b);
-}
-template <int V>
-__device__ __forceinline__ Lanes<V> operator+(const Lanes<V>& a, const Lanes<V>& b) {
-  return map([](auto x, auto y) { return x + y; }, a, b);
-}
-template <int V>
-__device__ __forceinline__ Lanes<V> one_less(const Lanes<V>& a) {
-  return map([](auto x) { return one_minus(x); }, a);
-}
-template <bool PRECISE, int V>
-__device__ __forceinline__ Lanes<V> sigmoids(const Lanes<V>& a) {
-  return map([](auto x) { return sigmoid_f<PRECISE>(x); }, a);
-}
-template <bool PRECISE, int V>
-__device__ __forceinline__ Lanes<V> tanhs(const Lanes<V>& a) {
-  return map([](auto x) { return tanh_f<PRECISE>(x); }, a);
-}
-template <bool PRECISE, int V>
-__device__ __forceinline__ Lanes<V> sigmoid_tanhs(const Lanes<V>& a, const Lanes<V>& b) {
-  return map([](auto x, auto y) { return sigmoid_tanh<PRECISE>(x, y); }, a, b);
-}
-
-template <int V>
-struct alignas(V == 1 ? 8 : 16) Run {  // the action c -> a c + b of a run of steps
-  Lanes<V> a, b;
+struct alignas(8 * V) Run {  // the action c -> a c + b of a run of steps
+  F<V> a, b;
 };
 
 // Reads V elements; those past the length are given as the step that changes nothing.
@@ -212,19 +156,14 @@ __device__ __forceinline__ Vec<T, V> constant_vec(uint32_t bits) {
   return v;
 }
 template <typename T, int V>
-__device__ __forceinline__ Lanes<V> widen(const Vec<T, V>& v) {
-  Lanes<V> r;
+__device__ __forceinline__ F<V> widen(const Vec<T, V>& v) {
+  float r[V];
 #pragma unroll
-  for (int i = 0; i < Lanes<V>::N; ++i) {
-    if constexpr (V == 1)
-      r.p[i] = F<1>::of(v.get(0));
-    else
-      r.p[i] = F<2>::of(v.get(2 * i), v.get(2 * i + 1));
-  }
-  return r;
+  for (int k = 0; k < V; ++k) r[k] = v.get(k);
+  return F<V>::of(r);
 }
 template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> narrow(const Lanes<V>& f) {
+__device__ __forceinline__ Vec<T, V> narrow(F<V> f) {
   float r[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) r[k] = f.get(k);
@@ -233,42 +172,41 @@ __device__ __forceinline__ Vec<T, V> narrow(const Lanes<V>& f) {
   return v;
 }
 template <int V>
-__device__ __forceinline__ Lanes<V> load_state(const float* p, int64_t at, bool live) {
+__device__ __forceinline__ F<V> load_state(const float* p, int64_t at, bool live) {
   float r[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) r[k] = live && p != nullptr ? p[at + k] : 0.0f;
-  Lanes<V> f;
-#pragma unroll
-  for (int i = 0; i < Lanes<V>::N; ++i) {
-    if constexpr (V == 1)
-      f.p[i] = F<1>::of(r[0]);
-    else
-      f.p[i] = F<2>::of(r[2 * i], r[2 * i + 1]);
-  }
-  return f;
+  return F<V>::of(r);
 }
 template <int V>
-__device__ __forceinline__ void store_state(float* p, int64_t at, const Lanes<V>& f) {
+__device__ __forceinline__ void store_state(float* p, int64_t at, F<V> f) {
 #pragma unroll
   for (int k = 0; k < V; ++k) p[at + k] = f.get(k);
 }
 
-// Where a thread stands.
+// Where a thread stands.  A CTA holds several groups of channels only with one segment (no exchange).
 template <int V>
 struct Place {
   int b, ch, cl, seg, rank, ranks, len;
-  bool live;  // its channels exist
+  int warp_seg, warp_ch;  // the warp's first segment and channel
+  bool live;              // its channels exist
   __device__ __forceinline__ Place(const ScanArgs& p, int cluster) {
     ranks = cluster;
     rank = blockIdx.x % cluster;
-    const int group = blockIdx.x / cluster;
     cl = threadIdx.x % p.cl;
-    seg = threadIdx.x / p.cl;
+    const int part = threadIdx.x / p.cl;
+    seg = part % p.seg;
+    const int group = blockIdx.x / cluster * p.groups + part / p.seg;
     b = group / p.ch_blocks;
-    ch = ((group % p.ch_blocks) * p.cl + cl) * V;
-    live = ch < p.H;
+    ch = ((group - b * p.ch_blocks) * p.cl + cl) * V;
+    warp_seg = seg - (int)(threadIdx.x & 31) / p.cl;
+    warp_ch = ch - cl * V;
+    live = b < p.B && ch < p.H;
     len = p.T;
-    if (p.lengths != nullptr) len = min(max(p.lengths[b], 0), p.T);
+    if (b >= p.B)
+      len = 0;
+    else if (p.lengths != nullptr)
+      len = min(max(p.lengths[b], 0), p.T);
   }
 };
 
@@ -280,12 +218,12 @@ struct Exchange {
   Run<V>* segs;   // [2][seg][cl]
   Run<V>* ranks;  // [2][kMaxCluster][cl]
 
-  __device__ __forceinline__ Lanes<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
-                                                 Lanes<V>& carry) const {
+  __device__ __forceinline__ F<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
+                                                 F<V>& carry) const {
     const int parity = turn & 1;
     Run<V>* const mine = segs + parity * p.seg * p.cl + at.cl;
     const int order = REVERSE ? p.seg - 1 - at.seg : at.seg;
-    Lanes<V> state = carry;
+    F<V> state = carry;
     if (at.ranks == 1) {
       if (p.seg == 1) {
         carry = fma(own.a, carry, own.b);
@@ -304,7 +242,7 @@ struct Exchange {
     mine[order * p.cl] = own;
     __syncthreads();
     // The run of the CTA's segments before this thread's, and of all of them.
-    Run<V> all{Lanes<V>::of(1.0f), Lanes<V>::of(0.0f)};
+    Run<V> all{F<V>::of(1.0f), F<V>::of(0.0f)};
     const auto fold = [&](const Run<V>& r) {
       all.b = fma(r.a, all.b, r.b);
       all.a = r.a * all.a;
@@ -329,8 +267,8 @@ struct Exchange {
   }
 };
 
-// K consecutive steps of V channels of NQ rows of gates (and, with dh, the gradient of h).  Steps from
-// the length on are given as the step that changes nothing: an infinite forget gate over zeros.
+// K consecutive steps of the four gates of V channels, `left` of them within the length.  Those past it
+// are given as the step that changes nothing: an infinite forget gate over zeros.
 template <typename T, int V, int K>
 __device__ __forceinline__ void load_steps(const T* from, int64_t stride, int H, bool live, int left,
                                            Vec<T, V> (&raw)[4][K]) {
@@ -351,59 +289,118 @@ __device__ __forceinline__ void load_steps(const T* from, int64_t stride, int H,
   }
 }
 
-// K: steps of a segment; the state entering every kSeg-th step is kept for the backward.
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
-  constexpr bool PRECISE = sizeof(T) == 4;
+// The gates (ROWS = 4) or the gradient of h (ROWS = 1) of a warp's segments on their way into shared
+// memory, 16 bytes a lane and copy (cp.async): word [step][row][lane] is what `lane` will read.  A warp reads
+// only what it copied, so no barrier is needed, and the copies for a turn fly while the turn before is
+// worked on without holding registers.  Steps past the length and channels past H arrive as zeros.
+template <typename T, int V, int K, int ROWS>
+struct Staged {
+  static constexpr int kWord = V * sizeof(T), kPieces = 32 * kWord / 16;  // 16-byte pieces of one [lane] row
+  static constexpr int kCopies = K * ROWS * kPieces / 32, kBytes = K * ROWS * 32 * kWord;
+  unsigned char* smem;  // this warp's
+  // `t`: first step of the warp's first segment; `from`: its row's first channel at step 0.
+  __device__ __forceinline__ void issue(const T* from, int64_t stride, int H, int cl, int ch0, int t, int len) const {
+    const int lane = threadIdx.x & 31, r = lane % kPieces, per_seg = cl * kWord / 16;
+    const int segment = r / per_seg, ch = (r - segment * per_seg) * (16 / (int)sizeof(T));
+    const bool live = ch0 + ch < H;
+    t += segment * K;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem) + lane * 16;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const int row = c * (32 / kPieces) + lane / kPieces, j = row / ROWS, q = row % ROWS;
+      const bool in = live && t + j < len;
+      const T* src = in ? from + (t + j) * stride + (int64_t)q * H + ch : from;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + c * 512), "l"(src), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+  }
+  __device__ __forceinline__ Vec<T, V> get(int j, int q) const {
+    return load_vec<T, V>(reinterpret_cast<const T*>(smem + ((j * ROWS + q) * 32 + (threadIdx.x & 31)) * kWord));
+  }
+};
+__device__ __forceinline__ void staged_wait() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+}
+
+// K: steps of a segment, kSeg, or fewer where the whole sequence is no longer.  The state entering
+// every segment is kept for the backward.
+template <typename T, int V, int K, bool STAGED>
+__global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : STAGED ? 5 : 4) scan_forward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+  constexpr bool PRECISE = sizeof(T) == 4, ONE = K < kSeg;  // ONE: one segment is the whole sequence
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
   const Exchange<V, false> exchange{reinterpret_cast<Run<V>*>(smem),
                                     reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
   // Distributed shared memory may be written once every CTA of the cluster has started.
-  if (cluster > 1) cg::this_cluster().sync();
+  if (!ONE && cluster > 1) cg::this_cluster().sync();
   const int tile = K * p.seg * cluster;
   const int turns = (at.len + tile - 1) / tile;
   const int kept = (p.T + kSeg - 1) / kSeg;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   T* h = static_cast<T*>(p.h) + at.b * p.h_sb + at.ch;
   const int64_t state_at = (int64_t)at.b * p.H + at.ch;
-  Lanes<V> carry = load_state<V>(p.c0, state_at, at.live);
+  F<V> carry = load_state<V>(p.c0, state_at, at.live);
   const int mine = (at.rank * p.seg + at.seg) * K;
+  // The next turn's gates are on their way during the exchange and the second pass: into shared
+  // memory, or into registers where those hold them.
+  constexpr bool AHEAD = !STAGED && K == kSeg && V * sizeof(T) <= 4;
+  const Staged<T, V, K, 4> staged{smem + p.stage_at + threadIdx.x / 32 * Staged<T, V, K, 4>::kBytes};
+  const int warp_t = (at.rank * p.seg + at.warp_seg) * K;
+  const T* const row = gates - at.ch + at.warp_ch;
   Vec<T, V> raw[4][K];
-  load_steps<T, V, K>(gates + mine * p.g_st, p.g_st, p.H, at.live, at.len - mine, raw);
+  if (STAGED && turns > 0) staged.issue(row, p.g_st, p.H, p.cl, at.warp_ch, warp_t, at.len);
+  if (AHEAD) load_steps<T, V, K>(gates + mine * p.g_st, p.g_st, p.H, at.live, at.len - mine, raw);
   for (int turn = 0; turn < turns; ++turn) {
     const int t0 = turn * tile + mine;
-    Lanes<V> f[K], u[K];
-    Run<V> own{Lanes<V>::of(1.0f), Lanes<V>::of(0.0f)};
+    if (STAGED) {
+      staged_wait();
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) raw[q][j] = staged.get(j, q);
+        if (t0 + j >= at.len) {
+          raw[1][j] = constant_vec<T, V>(infinity_bits<T>());
+        }
+      }
+    } else if (!AHEAD) {
+      load_steps<T, V, K>(gates + t0 * p.g_st, p.g_st, p.H, at.live, at.len - t0, raw);
+    }
+    F<V> f[K], u[K];
+    Run<V> own{F<V>::of(1.0f), F<V>::of(0.0f)};
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      f[j] = sigmoids<PRECISE>(widen<T, V>(raw[1][j]));
-      u[j] = sigmoid_tanhs<PRECISE>(widen<T, V>(raw[0][j]), widen<T, V>(raw[2][j]));
+      f[j] = sigmoid_f<PRECISE>(widen<T, V>(raw[1][j]));
+      u[j] = sigmoid_tanh<PRECISE>(widen<T, V>(raw[0][j]), widen<T, V>(raw[2][j]));
       own.b = j == 0 ? u[0] : fma(f[j], own.b, u[j]);
       own.a = j == 0 ? f[0] : own.a * f[j];
     }
-    // The next turn's gates are on their way during the exchange and the second pass.
     Vec<T, V> out_gate[K];
 #pragma unroll
     for (int j = 0; j < K; ++j) out_gate[j] = raw[3][j];
-    if (turn + 1 < turns)
+    if (STAGED && turn + 1 < turns) {
+      __syncwarp();
+      staged.issue(row, p.g_st, p.H, p.cl, at.warp_ch, warp_t + (turn + 1) * tile, at.len);
+    }
+    if (AHEAD && turn + 1 < turns)
       load_steps<T, V, K>(gates + (t0 + tile) * p.g_st, p.g_st, p.H, at.live, at.len - t0 - tile, raw);
-    Lanes<V> c = exchange(p, at, turn, own, carry);
+    F<V> c = ONE ? carry : exchange(p, at, turn, own, carry);
+    if (ONE) carry = fma(own.a, carry, own.b);
     if (!at.live) continue;
-    if (p.ckpt != nullptr && t0 < at.len && (K % kSeg == 0 || t0 % kSeg == 0))
+    if (p.ckpt != nullptr && t0 < at.len)
       store_state<V>(p.ckpt, ((int64_t)at.b * kept + t0 / kSeg) * p.H + at.ch, c);
     T* const to = h + t0 * p.h_st;
     if (t0 + K <= at.len) {
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         c = fma(f[j], c, u[j]);
-        store_vec<T, V>(to + j * p.h_st, narrow<T, V>(sigmoid_tanhs<PRECISE>(widen<T, V>(out_gate[j]), c)));
+        store_vec<T, V>(to + j * p.h_st, narrow<T, V>(sigmoid_tanh<PRECISE>(widen<T, V>(out_gate[j]), c)));
       }
     } else {
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         c = fma(f[j], c, u[j]);
-        const Vec<T, V> out = narrow<T, V>(sigmoid_tanhs<PRECISE>(widen<T, V>(out_gate[j]), c));
+        const Vec<T, V> out = narrow<T, V>(sigmoid_tanh<PRECISE>(widen<T, V>(out_gate[j]), c));
         if (t0 + j < p.T) store_vec<T, V>(to + j * p.h_st, t0 + j < at.len ? out : constant_vec<T, V>(0));
       }
     }
@@ -414,23 +411,29 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_
   if (at.rank == 0 && at.seg == 0) store_state<V>(p.c_n, state_at, carry);
 }
 
+// Two of the five values that a step keeps for the second pass wait in shared memory, where the registers
+// then leave room for a fifth CTA on an SM: one row of 65,536 steps, H = 512, bf16 takes 283 us against 396 us,
+// 64 x 1000 x 310 takes 120 us against 155 us.  Not for pairs of f32 channels, whose loads alone fill the
+// registers of five CTAs (64 x 2000 x 256: 251 us without, 328 us with).
 template <typename T, int V>
-__global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
-  constexpr bool PRECISE = sizeof(T) == 4;
-  constexpr int K = kSeg;
+constexpr bool kHeld = V * sizeof(T) <= 4;
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : kHeld<T, V> ? 5 : 4) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+  constexpr bool PRECISE = sizeof(T) == 4, ONE = K < kSeg, HELD = kHeld<T, V> && !ONE;  // ONE: one segment is the whole sequence
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
   const Exchange<V, true> exchange{reinterpret_cast<Run<V>*>(smem),
                                    reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
-  if (cluster > 1) cg::this_cluster().sync();
+  if (!ONE && cluster > 1) cg::this_cluster().sync();
   const int tile = K * p.seg * cluster;
   const int turns = (at.len + tile - 1) / tile;
-  const int kept = (p.T + K - 1) / K;
+  const int kept = (p.T + kSeg - 1) / kSeg;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   const T* dh = p.dh != nullptr ? static_cast<const T*>(p.dh) + at.b * p.h_sb + at.ch : nullptr;
   T* dg = static_cast<T*>(p.dgates) + at.b * p.d_sb + at.ch;
   const int64_t state_at = (int64_t)at.b * p.H + at.ch;
-  Lanes<V> carry = load_state<V>(p.dc_n, state_at, at.live);
+  F<V> carry = load_state<V>(p.dc_n, state_at, at.live);
+  F<V>* const held = reinterpret_cast<F<V>*>(smem + p.stage_at) + threadIdx.x;  // [2 K][kMaxThreads]
   for (int turn = 0; turn < turns; ++turn) {
     const int t0 = (turns - 1 - turn) * tile + (at.rank * p.seg + at.seg) * K;
     const int left = at.len - t0;
@@ -440,26 +443,26 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_
 #pragma unroll
     for (int j = 0; j < K; ++j)
       rdh[j] = at.live && j < left && dh != nullptr ? load_vec<T, V>(dh + (t0 + j) * p.h_st) : constant_vec<T, V>(0);
-    Lanes<V> c = load_state<V>(p.ckpt, ((int64_t)at.b * kept + t0 / K) * p.H + at.ch, at.live && left > 0);
+    F<V> c = load_state<V>(p.ckpt, ((int64_t)at.b * kept + t0 / kSeg) * p.H + at.ch, at.live && left > 0);
     // Per step: f, e and what dc is multiplied with in the gradients of i, f and g.
-    Lanes<V> f[K], e[K], wi[K], wf[K], wg[K];
+    F<V> f[K], e[K], wf[K], wi[HELD ? 1 : K], wg[HELD ? 1 : K];
     T* const to = dg + t0 * p.d_st;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const Lanes<V> si = sigmoids<PRECISE>(widen<T, V>(raw[0][j])), sf = sigmoids<PRECISE>(widen<T, V>(raw[1][j]));
-      const Lanes<V> g = tanhs<PRECISE>(widen<T, V>(raw[2][j])), so = sigmoids<PRECISE>(widen<T, V>(raw[3][j]));
+      const F<V> si = sigmoid_f<PRECISE>(widen<T, V>(raw[0][j])), sf = sigmoid_f<PRECISE>(widen<T, V>(raw[1][j]));
+      const F<V> g = tanh_f<PRECISE>(widen<T, V>(raw[2][j])), so = sigmoid_f<PRECISE>(widen<T, V>(raw[3][j]));
       f[j] = sf;
-      wf[j] = c * (sf * one_less(sf));
-      wi[j] = g * (si * one_less(si));
-      wg[j] = si * one_less(g * g);
+      wf[j] = c * (sf * one_minus(sf));
+      (HELD ? held[2 * j * kMaxThreads] : wi[HELD ? 0 : j]) = g * (si * one_minus(si));
+      (HELD ? held[(2 * j + 1) * kMaxThreads] : wg[HELD ? 0 : j]) = si * one_minus(g * g);
       c = fma(sf, c, si * g);
-      const Lanes<V> tc = tanhs<PRECISE>(c), dso = widen<T, V>(rdh[j]) * so;
-      e[j] = dso * one_less(tc * tc);
-      const Vec<T, V> d_o = narrow<T, V>(dso * tc * one_less(so));
+      const F<V> tc = tanh_f<PRECISE>(c), dso = widen<T, V>(rdh[j]) * so;
+      e[j] = dso * one_minus(tc * tc);
+      const Vec<T, V> d_o = narrow<T, V>(dso * tc * one_minus(so));
       if (whole) {
         if (at.live) store_vec<T, V>(to + j * p.d_st + 3 * (int64_t)p.H, d_o);
       } else {
-        if (j >= left) e[j] = Lanes<V>::of(0.0f);
+        if (j >= left) e[j] = F<V>::of(0.0f);
         if (at.live && t0 + j < p.T)
           store_vec<T, V>(to + j * p.d_st + 3 * (int64_t)p.H, j < left ? d_o : constant_vec<T, V>(0));
       }
@@ -470,29 +473,30 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_
       own.b = f[j] * (e[j] + own.b);
       own.a = own.a * f[j];
     }
-    Lanes<V> G = exchange(p, at, turn, own, carry);
+    F<V> G = ONE ? carry : exchange(p, at, turn, own, carry);
+    if (ONE) carry = fma(own.a, carry, own.b);
     if (!at.live) continue;
     if (whole) {
 #pragma unroll
       for (int j = K - 1; j >= 0; --j) {
-        const Lanes<V> dc = e[j] + G;
+        const F<V> dc = e[j] + G;
         G = f[j] * dc;
         T* const at_j = to + j * p.d_st;
-        store_vec<T, V>(at_j, narrow<T, V>(dc * wi[j]));
+        store_vec<T, V>(at_j, narrow<T, V>(dc * (HELD ? held[2 * j * kMaxThreads] : wi[HELD ? 0 : j])));
         store_vec<T, V>(at_j + p.H, narrow<T, V>(dc * wf[j]));
-        store_vec<T, V>(at_j + 2 * (int64_t)p.H, narrow<T, V>(dc * wg[j]));
+        store_vec<T, V>(at_j + 2 * (int64_t)p.H, narrow<T, V>(dc * (HELD ? held[(2 * j + 1) * kMaxThreads] : wg[HELD ? 0 : j])));
       }
     } else {
 #pragma unroll
       for (int j = K - 1; j >= 0; --j) {
-        const Lanes<V> dc = e[j] + G;
+        const F<V> dc = e[j] + G;
         G = f[j] * dc;
         const Vec<T, V> none = constant_vec<T, V>(0);
         T* const at_j = to + j * p.d_st;
         if (t0 + j < p.T) {
-          store_vec<T, V>(at_j, j < left ? narrow<T, V>(dc * wi[j]) : none);
+          store_vec<T, V>(at_j, j < left ? narrow<T, V>(dc * (HELD ? held[2 * j * kMaxThreads] : wi[HELD ? 0 : j])) : none);
           store_vec<T, V>(at_j + p.H, j < left ? narrow<T, V>(dc * wf[j]) : none);
-          store_vec<T, V>(at_j + 2 * (int64_t)p.H, j < left ? narrow<T, V>(dc * wg[j]) : none);
+          store_vec<T, V>(at_j + 2 * (int64_t)p.H, j < left ? narrow<T, V>(dc * (HELD ? held[(2 * j + 1) * kMaxThreads] : wg[HELD ? 0 : j])) : none);
         }
       }
     }
@@ -505,61 +509,77 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 128 ? 4 : 2) scan_
   if (p.dc0 != nullptr && at.rank == 0 && at.seg == 0) store_state<V>(p.dc0, state_at, carry);
 }
 
-// How the work is split: channel lanes to fill a warp where H allows, then time segments up to
-// the CTA's threads, then a cluster where the CTAs would not fill the GPU; never more segments
-// than the sequence has.
+// How the work is split.  A CTA has 128 threads of up to 128 registers (four on an SM): 32 channel
+// lanes (128 bytes of a 16-bit row) by four segments.  Where that gives fewer than 512 CTAs, a CTA takes
+// fewer channels and more segments, down to rows of 32 bytes, and then the CTAs of a cluster share a
+// channel; there are never more segments than the sequence has.  Where there are warps enough without
+// splitting time, every warp walks its row alone.
 struct Plan {
-  int cl, seg, cluster, ch_blocks;
+  int cl, seg, groups, cluster, ch_blocks;
 };
 
-Plan make_plan(int B, int T, int H, int V, int K) {
+Plan make_plan(int B, int T, int H, int V, int K, int size, bool backward) {
   Plan p;
-  const int lanes = (H + V - 1) / V;
+  const int lanes = (H + V - 1) / V, segments = std::max(1, (T + K - 1) / K);
   p.cl = 1;
-  while (p.cl < 32 && p.cl < lanes) p.cl *= 2;
-  p.ch_blocks = (lanes + p.cl - 1) / p.cl;
-  const int segments = std::max(1, (T + K - 1) / K);
+  const int narrowest = (int64_t)H * size % 32 == 0 ? 32 : 64;  // bytes of a row that cost whole sectors
+  const int widest = backward && segments >= 8 && narrowest == 32 && V * size <= 4 ? 16 : 32;
+  while (p.cl < widest && p.cl < lanes) p.cl *= 2;
+  const auto blocks = [&] { return (int64_t)B * ((lanes + p.cl - 1) / p.cl); };
+  while (p.cl * V * size / 2 >= narrowest && blocks() < kWanted && kMaxThreads / p.cl < segments) p.cl /= 2;
   p.seg = 1;
-  while (p.seg * p.cl < kMaxThreads && p.seg < segments) p.seg *= 2;
+  if (blocks() * p.cl < 32 * kAlone || p.cl < 16)
+    while (p.seg * p.cl < kMaxThreads && p.seg < segments) p.seg *= 2;
   p.cluster = 1;
-  const int64_t groups = (int64_t)B * p.ch_blocks;
-  while (p.cluster < kMaxCluster && groups * p.cluster < 2 * kSMs && p.seg * p.cluster < segments) p.cluster *= 2;
+  while (p.cluster < kMaxCluster && blocks() * p.cluster < kWanted && p.seg * p.cluster < segments) p.cluster *= 2;
+  p.groups = p.seg == 1 ? std::max(1, kMaxThreads / p.cl) : 1;
+  p.ch_blocks = (lanes + p.cl - 1) / p.cl;
   return p;
 }
 
-template <typename T, int V, int K>
+// STAGED: V channels of a lane that come through shared memory, 16 bytes a copy.
+template <typename T, int V, int K, bool STAGED>
 int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
-  const Plan plan = make_plan(a.B, a.T, a.H, V, K);
+  const Plan plan = make_plan(a.B, a.T, a.H, V, K, (int)sizeof(T), backward);
   a.cl = plan.cl;
   a.seg = plan.seg;
+  a.groups = plan.groups;
   a.ch_blocks = plan.ch_blocks;
-  const int64_t ctas = (int64_t)a.B * plan.ch_blocks * plan.cluster;
-  if (ctas > 0x7fffffff) {
+  const int64_t ctas = ((int64_t)a.B * plan.ch_blocks + plan.groups - 1) / plan.groups * plan.cluster;
+  if ((int64_t)a.B * plan.ch_blocks > 0x7fffffff - kMaxThreads || ctas > 0x7fffffff) {
     set_error("gated scan: batch * hidden is too large for one launch");
     return PLSTM_ENOTSUP;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(plan.cl * plan.seg);
-  cfg.dynamicSmemBytes = (size_t)2 * (plan.seg + kMaxCluster) * plan.cl * sizeof(Run<V>);
+  cfg.blockDim = dim3(plan.cl * plan.seg * plan.groups);
+  a.stage_at = plan.seg > 1 ? (int)(2 * (plan.seg + kMaxCluster) * plan.cl * sizeof(Run<V>)) : 0;
+  const bool staged = STAGED && !backward && plan.cluster > 1;
+  cfg.dynamicSmemBytes = a.stage_at + (backward ? (kHeld<T, V> && K == kSeg ? 2 * K * kMaxThreads * sizeof(F<V>) : 0)
+                                       : staged ? cfg.blockDim.x / 32 * Staged<T, V, K, 4>::kBytes
+                                                : 0);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = plan.cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = plan.cluster > 1 ? 1 : 0;
   const auto go = [&](auto kernel) -> int32_t {
     if (plan.cluster > 8)  // beyond the portable size: has to be allowed for the kernel
       PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (cfg.dynamicSmemBytes > 48 * 1024)
+      PLSTM_TRY_CUDA(
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
     PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan.cluster));
     note_launches(1);
     return PLSTM_OK;
   };
-  if constexpr (K == kSeg) {
-    if (backward) return go(scan_backward_kernel<T, V>);
+  if (backward) return go(scan_backward_kernel<T, V, K>);
+  if constexpr (STAGED) {
+    if (staged) return go(scan_forward_kernel<T, V, K, true>);
   }
-  return go(scan_forward_kernel<T, V, K>);
+  return go(scan_forward_kernel<T, V, K, false>);
 }
 
 // Every access of V channels is aligned to V elements.
@@ -570,15 +590,21 @@ bool aligned_lanes(int dtype, const ScanArgs& a, int V) {
   return aligned_to(a.gates, bytes) && aligned_to(a.h, bytes) && aligned_to(a.dh, bytes) && aligned_to(a.dgates, bytes);
 }
 
+// A single step, or up to four, would waste most of a segment of eight.
+template <typename T, int V>
+int32_t dispatch_steps(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
+  if (a.T <= 1) return launch<T, V, 1, false>(backward, a, s);
+  if (a.T <= 4) return launch<T, V, 4, false>(backward, a, s);
+  if constexpr (V == 2 && sizeof(T) == 2) {
+    if (aligned_lanes(dtype, a, 16 / sizeof(T)) && a.H >= 64) return launch<T, V, kSeg, true>(backward, a, s);
+  }
+  return launch<T, V, kSeg, false>(backward, a, s);
+}
+
 template <typename T>
 int32_t dispatch_type(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    // Four channels halve the loads, stores and addresses of an element; four steps then fill the
-    // registers that eight do with two channels.
-    if (!backward && aligned_lanes(dtype, a, 4)) return launch<T, 4, 4>(false, a, s);
-  }
-  if (aligned_lanes(dtype, a, 2)) return launch<T, 2, kSeg>(backward, a, s);
-  return launch<T, 1, kSeg>(backward, a, s);
+  return aligned_lanes(dtype, a, 2) ? dispatch_steps<T, 2>(backward, dtype, a, s)
+                                    : dispatch_steps<T, 1>(backward, dtype, a, s);
 }
 
 int32_t dispatch(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {

@@ -289,14 +289,21 @@ __device__ __forceinline__ void load_steps(const T* from, int64_t stride, int H,
   }
 }
 
-// The gates (ROWS = 4) or the gradient of h (ROWS = 1) of a warp's segments on their way into shared
-// memory, 16 bytes a lane and copy (cp.async): word [step][row][lane] is what `lane` will read.  A warp reads
-// only what it copied, so no barrier is needed, and the copies for a turn fly while the turn before is
-// worked on without holding registers.  Steps past the length and channels past H arrive as zeros.
-template <typename T, int V, int K, int ROWS>
+// The gates of a warp's segments on their way into shared memory, 16 bytes a lane and copy (cp.async):
+// word [step][gate][lane] is what `lane` will read.  A warp reads only what it copied, so no barrier is
+// needed, and the copies for a turn fly while the turn before is worked on without holding registers.
+// Steps past the length and channels past H arrive as zeros.  The forward stages in clusters, where a turn
+// is long and the warps are few (one row of 65,536 steps, H = 512, bf16: 178 us against 224 us with the next
+// turn in registers); elsewhere the detour costs more than it hides (B = 512, T = 1000, H = 128, f16: 185 us
+// against 168 us), and so it does in the backward.
+template <typename T, int V, int K>
 struct Staged {
-  static constexpr int kWord = V * sizeof(T), kPieces = 32 * kWord / 16;  // 16-byte pieces of one [lane] row
-  static constexpr int kCopies = K * ROWS * kPieces / 32, kBytes = K * ROWS * 32 * kWord;
+  enum : int {
+    kWord = V * (int)sizeof(T),
+    kPieces = 32 * kWord / 16,  // 16-byte pieces of one [lane] row
+    kCopies = K * 4 * kPieces / 32,
+    kBytes = K * 4 * 32 * kWord,
+  };
   unsigned char* smem;  // this warp's
   // `t`: first step of the warp's first segment; `from`: its row's first channel at step 0.
   __device__ __forceinline__ void issue(const T* from, int64_t stride, int H, int cl, int ch0, int t, int len) const {
@@ -307,7 +314,7 @@ struct Staged {
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem) + lane * 16;
 #pragma unroll
     for (int c = 0; c < kCopies; ++c) {
-      const int row = c * (32 / kPieces) + lane / kPieces, j = row / ROWS, q = row % ROWS;
+      const int row = c * (32 / kPieces) + lane / kPieces, j = row / 4, q = row % 4;
       const bool in = live && t + j < len;
       const T* src = in ? from + (t + j) * stride + (int64_t)q * H + ch : from;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + c * 512), "l"(src), "r"(in ? 16 : 0)
@@ -315,7 +322,7 @@ struct Staged {
     }
   }
   __device__ __forceinline__ Vec<T, V> get(int j, int q) const {
-    return load_vec<T, V>(reinterpret_cast<const T*>(smem + ((j * ROWS + q) * 32 + (threadIdx.x & 31)) * kWord));
+    return load_vec<T, V>(reinterpret_cast<const T*>(smem + ((j * 4 + q) * 32 + (threadIdx.x & 31)) * kWord));
   }
 };
 __device__ __forceinline__ void staged_wait() {
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : STAGED ? 5 : 4) sc
   // The next turn's gates are on their way during the exchange and the second pass: into shared
   // memory, or into registers where those hold them.
   constexpr bool AHEAD = !STAGED && K == kSeg && V * sizeof(T) <= 4;
-  const Staged<T, V, K, 4> staged{smem + p.stage_at + threadIdx.x / 32 * Staged<T, V, K, 4>::kBytes};
+  const Staged<T, V, K> staged{smem + p.stage_at + threadIdx.x / 32 * Staged<T, V, K>::kBytes};
   const int warp_t = (at.rank * p.seg + at.warp_seg) * K;
   const T* const row = gates - at.ch + at.warp_ch;
   Vec<T, V> raw[4][K];
@@ -509,6 +516,56 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : kHeld<T, V> ? 5 : 
   if (p.dc0 != nullptr && at.rank == 0 && at.seg == 0) store_state<V>(p.dc0, state_at, carry);
 }
 
+// One step of a batch of streams: a thread takes V channels of one row, nothing is exchanged.
+template <typename T, int V>
+__global__ void __launch_bounds__(kMaxThreads) scan_step_kernel(const __grid_constant__ ScanArgs p) {
+  constexpr bool PRECISE = sizeof(T) == 4;
+  constexpr int W = V == 1 ? 1 : 2;
+  const int ch = (blockIdx.x * kMaxThreads + threadIdx.x) * V;
+  if (ch >= p.H) return;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const bool in = p.lengths == nullptr || p.lengths[b] > 0;
+    const T* const from = static_cast<const T*>(p.gates) + b * p.g_sb + ch;
+    const int64_t at = (int64_t)b * p.H + ch;
+    Vec<T, V> raw[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      raw[q] = in ? load_vec<T, V>(from + (int64_t)q * p.H) : constant_vec<T, V>(q == 1 ? infinity_bits<T>() : 0);
+    float c[V], h[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      c[k] = p.c0 != nullptr ? p.c0[at + k] : 0.0f;
+      if (p.ckpt != nullptr) p.ckpt[at + k] = c[k];
+    }
+#pragma unroll
+    for (int i = 0; i < V / W; ++i) {
+      F<W> gate[4], state;
+      if constexpr (V == 1) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) gate[q] = F<1>::of(raw[q].get(0));
+        state = F<1>::of(c[0]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) gate[q] = F<2>::of(raw[q].get(2 * i), raw[q].get(2 * i + 1));
+        state = F<2>::of(c[2 * i], c[2 * i + 1]);
+      }
+      const F<W> f = sigmoid_f<PRECISE>(gate[1]), u = sigmoid_tanh<PRECISE>(gate[0], gate[2]);
+      state = fma(f, state, u);
+      const F<W> o = sigmoid_tanh<PRECISE>(gate[3], state);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        c[W * i + k] = state.get(k);
+        h[W * i + k] = o.get(k);
+      }
+    }
+    Vec<T, V> out;
+    out.set(h);
+    store_vec<T, V>(static_cast<T*>(p.h) + b * p.h_sb + ch, in ? out : constant_vec<T, V>(0));
+#pragma unroll
+    for (int k = 0; k < V; ++k) p.c_n[at + k] = c[k];
+  }
+}
+
 // How the work is split.  A CTA has 128 threads of up to 128 registers (four on an SM): 32 channel
 // lanes (128 bytes of a 16-bit row) by four segments.  Where that gives fewer than 512 CTAs, a CTA takes
 // fewer channels and more segments, down to rows of 32 bytes, and then the CTAs of a cluster share a
@@ -556,7 +613,7 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
   a.stage_at = plan.seg > 1 ? (int)(2 * (plan.seg + kMaxCluster) * plan.cl * sizeof(Run<V>)) : 0;
   const bool staged = STAGED && !backward && plan.cluster > 1;
   cfg.dynamicSmemBytes = a.stage_at + (backward ? (kHeld<T, V> && K == kSeg ? 2 * K * kMaxThreads * sizeof(F<V>) : 0)
-                                       : staged ? cfg.blockDim.x / 32 * Staged<T, V, K, 4>::kBytes
+                                       : staged ? cfg.blockDim.x / 32 * Staged<T, V, K>::kBytes
                                                 : 0);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -579,7 +636,8 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
   if constexpr (STAGED) {
     if (staged) return go(scan_forward_kernel<T, V, K, true>);
   }
-  return go(scan_forward_kernel<T, V, K, false>);
+  if constexpr (K > 1) return go(scan_forward_kernel<T, V, K, false>);
+  return PLSTM_EINVAL;  // one step forward is launch_step's
 }
 
 // Every access of V channels is aligned to V elements.
@@ -590,10 +648,19 @@ bool aligned_lanes(int dtype, const ScanArgs& a, int V) {
   return aligned_to(a.gates, bytes) && aligned_to(a.h, bytes) && aligned_to(a.dh, bytes) && aligned_to(a.dgates, bytes);
 }
 
+template <typename T, int V>
+int32_t launch_step(const ScanArgs& a, cudaStream_t s) {
+  const dim3 grid((a.H + V * kMaxThreads - 1) / (V * kMaxThreads), std::min(a.B, 65535));
+  scan_step_kernel<T, V><<<grid, std::min(kMaxThreads, ((a.H + V - 1) / V + 31) / 32 * 32), 0, s>>>(a);
+  PLSTM_TRY_CUDA(cudaGetLastError());
+  note_launches(1);
+  return PLSTM_OK;
+}
+
 // A single step, or up to four, would waste most of a segment of eight.
 template <typename T, int V>
 int32_t dispatch_steps(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
-  if (a.T <= 1) return launch<T, V, 1, false>(backward, a, s);
+  if (backward && a.T == 1) return launch<T, V, 1, false>(true, a, s);
   if (a.T <= 4) return launch<T, V, 4, false>(backward, a, s);
   if constexpr (V == 2 && sizeof(T) == 2) {
     if (aligned_lanes(dtype, a, 16 / sizeof(T)) && a.H >= 64) return launch<T, V, kSeg, true>(backward, a, s);
@@ -603,6 +670,7 @@ int32_t dispatch_steps(bool backward, int dtype, const ScanArgs& a, cudaStream_t
 
 template <typename T>
 int32_t dispatch_type(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
+  if (!backward && a.T == 1) return aligned_lanes(dtype, a, 4) ? launch_step<T, 4>(a, s) : launch_step<T, 1>(a, s);
   return aligned_lanes(dtype, a, 2) ? dispatch_steps<T, 2>(backward, dtype, a, s)
                                     : dispatch_steps<T, 1>(backward, dtype, a, s);
 }

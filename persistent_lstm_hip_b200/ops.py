@@ -31,6 +31,17 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
     lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
+def _first_order(backward):
+    """once_differentiable, whose bookkeeping only a backward that is itself recorded needs."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 # What depends on shapes, strides and types alone (checks, descriptors, sizes) is worked out once for
 # each combination and found again by it in these bounded caches.
 _plan = functools.lru_cache(maxsize=512)
@@ -96,7 +107,7 @@ class _GatedScan(torch.autograd.Function):
         return h, c_n
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dh, dc_n):
         gates, lengths, ckpt = ctx.saved_tensors
         if dh is not None and dh.stride(2) != 1:
@@ -204,7 +215,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, drop, residual, x.dtype if residual is None else residual.dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         drop, dtype = ctx.args
         ctx.saved_tensors
@@ -344,7 +355,7 @@ class _LayerNorm(torch.autograd.Function):
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         eps, w_dtype = ctx.args
@@ -364,7 +375,7 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
         return (y, z) if x.dim() == 2 else (y.view(x.shape), z.view(x.shape))
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dz):
         z, weight, stats, _ = ctx.saved_tensors
         drop, eps, x_dtype, w_dtype = ctx.args

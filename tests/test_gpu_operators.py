@@ -600,3 +600,16 @@ def test_regressor_learns(cuda_device):
         losses.append(float(loss.detach()))
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
     assert losses[-1] < 0.25 * losses[0], losses[::10]
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    """Differentiating a gradient again is an error, never a silently wrong number; a recorded
+    backward alone is not."""
+    d = cuda_device
+    x, g = _randn(4, 16, dtype=F32, dev=d).requires_grad_(True), _gates(2, 5, 4, F32, d).requires_grad_(True)
+    for y, v in ((plstm.layer_norm(x), x), (plstm.dropout(x, 0.5, 1), x), (plstm.gated_scan(g)[0], g),
+                 (plstm.dropout_add_layer_norm(x, x * 2)[0], x)):
+        (d1,) = torch.autograd.grad((y * y).sum(), v, create_graph=True)
+        assert torch.isfinite(d1).all()
+        with pytest.raises(RuntimeError, match="once_differentiable|differentiated twice"):
+            d1.sum().backward()

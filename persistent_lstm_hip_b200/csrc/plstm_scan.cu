@@ -184,11 +184,13 @@ __device__ __forceinline__ void store_state(float* p, int64_t at, F<V> f) {
   for (int k = 0; k < V; ++k) p[at + k] = f.get(k);
 }
 
-// Where a thread stands.  A CTA holds several groups of channels only with one segment (no exchange).
+// Where a thread stands.  The groups of channels that share a CTA with an exchange (and so its barriers)
+// walk the whole sequence together; a group on its own stops at its length.
 template <int V>
 struct Place {
   int b, ch, cl, seg, rank, ranks, len;
   int warp_seg, warp_ch;  // the warp's first segment and channel
+  int local, span;        // the group's place in the CTA, the steps it walks
   bool live;              // its channels exist
   __device__ __forceinline__ Place(const ScanArgs& p, int cluster) {
     ranks = cluster;
@@ -196,7 +198,8 @@ struct Place {
     cl = threadIdx.x % p.cl;
     const int part = threadIdx.x / p.cl;
     seg = part % p.seg;
-    const int group = blockIdx.x / cluster * p.groups + part / p.seg;
+    local = part / p.seg;
+    const int group = blockIdx.x / cluster * p.groups + local;
     b = group / p.ch_blocks;
     ch = ((group - b * p.ch_blocks) * p.cl + cl) * V;
     warp_seg = seg - (int)(threadIdx.x & 31) / p.cl;
@@ -207,6 +210,7 @@ struct Place {
       len = 0;
     else if (p.lengths != nullptr)
       len = min(max(p.lengths[b], 0), p.T);
+    span = p.groups > 1 && p.seg > 1 ? p.T : len;
   }
 };
 
@@ -215,7 +219,7 @@ struct Place {
 // run.  Runs are folded in running order (backward: from the last segment and rank to the first).
 template <int V, bool REVERSE>
 struct Exchange {
-  Run<V>* segs;   // [2][seg][cl]
+  Run<V>* segs;   // [2][seg][cl] of the group
   Run<V>* ranks;  // [2][kMaxCluster][cl]
 
   __device__ __forceinline__ F<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
@@ -337,12 +341,12 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : STAGED ? 5 : 4) sc
   constexpr bool PRECISE = sizeof(T) == 4, ONE = K < kSeg;  // ONE: one segment is the whole sequence
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
-  const Exchange<V, false> exchange{reinterpret_cast<Run<V>*>(smem),
-                                    reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
+  const Exchange<V, false> exchange{reinterpret_cast<Run<V>*>(smem) + at.local * 2 * p.seg * p.cl,
+                                    reinterpret_cast<Run<V>*>(smem) + 2 * p.groups * p.seg * p.cl};
   // Distributed shared memory may be written once every CTA of the cluster has started.
   if (!ONE && cluster > 1) cg::this_cluster().sync();
   const int tile = K * p.seg * cluster;
-  const int turns = (at.len + tile - 1) / tile;
+  const int turns = (at.span + tile - 1) / tile;
   const int kept = (p.T + kSeg - 1) / kSeg;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   T* h = static_cast<T*>(p.h) + at.b * p.h_sb + at.ch;
@@ -429,11 +433,11 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : kHeld<T, V> ? 5 : 
   constexpr bool PRECISE = sizeof(T) == 4, ONE = K < kSeg, HELD = kHeld<T, V> && !ONE;  // ONE: one segment is the whole sequence
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
-  const Exchange<V, true> exchange{reinterpret_cast<Run<V>*>(smem),
-                                   reinterpret_cast<Run<V>*>(smem) + 2 * p.seg * p.cl};
+  const Exchange<V, true> exchange{reinterpret_cast<Run<V>*>(smem) + at.local * 2 * p.seg * p.cl,
+                                   reinterpret_cast<Run<V>*>(smem) + 2 * p.groups * p.seg * p.cl};
   if (!ONE && cluster > 1) cg::this_cluster().sync();
   const int tile = K * p.seg * cluster;
-  const int turns = (at.len + tile - 1) / tile;
+  const int turns = (at.span + tile - 1) / tile;
   const int kept = (p.T + kSeg - 1) / kSeg;
   const T* gates = static_cast<const T*>(p.gates) + at.b * p.g_sb + at.ch;
   const T* dh = p.dh != nullptr ? static_cast<const T*>(p.dh) + at.b * p.h_sb + at.ch : nullptr;
@@ -589,7 +593,12 @@ Plan make_plan(int B, int T, int H, int V, int K, int size, bool backward) {
     while (p.seg * p.cl < kMaxThreads && p.seg < segments) p.seg *= 2;
   p.cluster = 1;
   while (p.cluster < kMaxCluster && blocks() * p.cluster < kWanted && p.seg * p.cluster < segments) p.cluster *= 2;
-  p.groups = p.seg == 1 ? std::max(1, kMaxThreads / p.cl) : 1;
+  // A long sequence of few channels: sectors are wasted rather than SMs.
+  while (p.cluster == kMaxCluster && p.cl > 4 && blocks() * p.cluster < kWanted && p.seg * p.cluster < segments) {
+    p.cl /= 2;
+    p.seg *= 2;
+  }
+  p.groups = p.cluster == 1 ? std::max(1, kMaxThreads / (p.cl * p.seg)) : 1;
   p.ch_blocks = (lanes + p.cl - 1) / p.cl;
   return p;
 }
@@ -610,7 +619,7 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(plan.cl * plan.seg * plan.groups);
-  a.stage_at = plan.seg > 1 ? (int)(2 * (plan.seg + kMaxCluster) * plan.cl * sizeof(Run<V>)) : 0;
+  a.stage_at = plan.seg > 1 ? (int)((2 * plan.groups * plan.seg + 2 * kMaxCluster) * plan.cl * sizeof(Run<V>)) : 0;
   const bool staged = STAGED && !backward && plan.cluster > 1;
   cfg.dynamicSmemBytes = a.stage_at + (backward ? (kHeld<T, V> && K == kSeg ? 2 * K * kMaxThreads * sizeof(F<V>) : 0)
                                        : staged ? cfg.blockDim.x / 32 * Staged<T, V, K>::kBytes

@@ -537,15 +537,22 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __r
   if (threadIdx.x == 0 && c < cols && out != nullptr) store_any(out, w_dtype, c, s);
 }
 
-// Chunks a thread takes: enough to spread a row's fixed costs (sums, barriers, square root) over,
-// as far as the registers hold them.
+// Chunks a thread takes: enough to spread a row's fixed costs (sums, barriers, square root) over, as
+// far as the registers hold them.  Measured at 65536 x 1024 bf16: the forward takes 52 us with four and
+// 60 us with two; the backward 87 us with two (their sums of weight gradients are registers) and
+// 103 us with one.  A few rows are over before that matters, and one chunk is the shortest way
+// (backward of 16 x 512: 6.7 us with one, 9.0 us with two).  The fused forward would rather have two
+// (33000 x 1001: 122 us against 146 us), but it sums in the plain one's order, so that both give the
+// same bits.
 Split make_split(const plstm_norm_desc& d, bool whole, bool backward) {
   Split s;
   const int chunks = whole ? d.cols / 8 : chunk_columns(d.cols);
-  const bool f32 = d.x_dtype == PLSTM_F32;
-  s.ch = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
-  if (f32 && chunks <= 513) s.ch = std::min(s.ch, 2);
-  if (backward) s.ch = chunks <= 48 ? 1 : chunks <= 513 ? 2 : 4;
+  if (backward) {
+    const bool few = chunks <= 257 && d.rows * chunks <= (int64_t)kSMs * kTeamBlock * 4;
+    s.ch = chunks <= 48 || few ? 1 : chunks <= 513 ? 2 : 4;
+  } else {
+    s.ch = chunks <= 32 ? 1 : chunks <= (d.x_dtype == PLSTM_F32 ? 513 : 64) ? 2 : 4;
+  }
   const int threads = (chunks + s.ch - 1) / s.ch;
   if (threads >= 32) {
     s.tpr = (threads + 31) / 32 * 32;

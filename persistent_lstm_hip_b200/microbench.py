@@ -15,6 +15,11 @@
         The dependent-step latency probe (plstm_diag_step_latency): one wavefront
         layer-step's dependency chain alone, cycles and microseconds per step and
         its phases; the latency floor of the roofline.
+    python -m persistent_lstm_hip_b200.microbench gated [--hidden 128 --layers 4 --batch 512
+            --seq 1000 --input 5 --dtype bf16 --streams 16]
+        The training and streaming operators together, as GatedScanRegressor runs them: one
+        training step (forward, loss, backward, SGD update; dropout 0.2) and one streaming
+        step of `streams` streams, ms each.
 """
 from __future__ import annotations
 
@@ -157,6 +162,36 @@ def forward(args) -> dict:
             "kernel_ms": k_ms.value / max(n.value, 1), "seq_timesteps_per_s": steps / (ms / 1e3)}
 
 
+def gated(args) -> dict:
+    from .gated import GatedScanRegressor
+
+    dev = torch.device("cuda:0")
+    dt = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[args.dtype]
+    torch.manual_seed(0)
+    model = GatedScanRegressor(args.input, args.hidden, 24, args.layers).to(dev, dt)
+    opt = torch.optim.SGD(model.parameters(), lr=1e-3)
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(args.batch, args.seq, args.input, generator=gen).to(dev, dt)
+    target = torch.randn(args.batch, args.seq, 24, generator=gen).to(dev, dt)
+
+    def train():
+        opt.zero_grad()
+        out, _ = model(x)
+        ((out - target).float() ** 2).mean().backward()
+        opt.step()
+
+    model.train()
+    train_ms = _time(train, args.iters, 3)
+    model.eval()
+    state = model.init_state(args.streams)
+    xs = x[:1, 0].expand(args.streams, -1).contiguous()
+    step_ms = _time(lambda: model.step(xs, state), 10 * args.iters, 10)
+    return {"model": "GatedScanRegressor", "hidden": args.hidden, "layers": args.layers, "batch": args.batch,
+            "seq": args.seq, "dtype": args.dtype, "train_ms": train_ms,
+            "train_seq_timesteps_per_s": args.batch * args.seq / (train_ms / 1e3), "streams": args.streams,
+            "stream_step_ms": step_ms}
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="cmd", required=True)
@@ -184,8 +219,17 @@ def main() -> None:
     pr.add_argument("--rows", type=int, choices=[16, 32], default=16)
     pr.add_argument("--steps", type=int, default=20000)
     pr.add_argument("--variant", type=int, default=0, help="bits of plstm_diag_step_latency's variants")
+    ga = sub.add_parser("gated")
+    ga.add_argument("--hidden", type=int, default=128)
+    ga.add_argument("--layers", type=int, default=4)
+    ga.add_argument("--batch", type=int, default=512)
+    ga.add_argument("--seq", type=int, default=1000)
+    ga.add_argument("--input", type=int, default=5)
+    ga.add_argument("--dtype", choices=["f16", "bf16", "f32"], default="bf16")
+    ga.add_argument("--streams", type=int, default=16)
+    ga.add_argument("--iters", type=int, default=5)
     args = ap.parse_args()
-    print(json.dumps({"gemm": gemm, "step": step, "forward": forward, "probe": probe}[args.cmd](args)))
+    print(json.dumps({"gemm": gemm, "step": step, "forward": forward, "probe": probe, "gated": gated}[args.cmd](args)))
 
 
 if __name__ == "__main__":

@@ -15,8 +15,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // A thread takes kUnroll groups of eight elements a turn, a CTA's apart, and issues all their loads
-// before it draws: with one 16-byte load in flight a thread the kernel waited on memory
-// (82 us for 65.5 M f16 elements, floor 40).
+// before it draws: with one 16-byte load in flight a thread the kernel waited on memory (68 to 69 us
+// for 65.5 M f16 elements against 64 us; two groups take 65 to 69 us).  64 us is 63 % of the measured
+// bandwidth: 20 widening products a Philox call keep the multiplier 62 % busy, issue is 57 %.
 constexpr int kUnroll = 4;
 
 template <typename T>

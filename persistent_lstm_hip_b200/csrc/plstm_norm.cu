@@ -7,6 +7,13 @@
 //   dv = rstd (g - mean(g) - xh mean(g xh)) [+ dz],  dw = sum over rows of dy xh,  db = sum of dy.
 // The weight gradients are summed per thread over the rows its CTA visits, then over the
 // CTA's row groups, then over the CTAs by a second kernel: a fixed order, no atomics.
+//
+// Both directions are bound by instruction issue before memory.  Measured at 65536 x 1024 bf16 with f32
+// weights: forward 53 us, 78 % of the measured 6.54 TB/s (14 instructions an element); backward with the
+// weight gradients 86 us, 71 % (27 an element).  With residual and dropout at 131072 x 512: 126 and 161 us, 65 %
+// and 64 % (Philox adds 11.5 an element); with f32 throughout at 65536 x 512: 88 and 113 us, 93 % and 91 %.
+// Rows 1001 wide (33000 of them): 57 and 108 us against 27 and 44 us that their bytes would take at the 1024's rate:
+// the masked ends and the columns' places cost instructions.
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>

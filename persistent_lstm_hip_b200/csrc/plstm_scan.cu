@@ -15,9 +15,16 @@
 // steps again out of registers to write h.  The input is read once and the waits are the
 // hardware's barriers.
 //
+// Measured (GPU time, of the measured 6.54 TB/s): forward 169 us for B = 512, T = 1000, H = 128, f16, 59 % (the
+// special-function unit is 68 % busy with its eight instructions an element, the issue slots 59 %); 181 us for
+// one row of 65,536 steps of H = 512, bf16, 28 % (32 turns of a cluster exchange each); 228 us for 1024 rows of
+// 200 to 1000 steps, 59 %.
+//
 // Backward, with e_t = dh_t o_t (1 - tanh(c_t)^2): dc_t = e_t + G_t, G_{t-1} = f_t dc_t, where
 // G enters the last step as dc_n and leaves the first as dc0: the same composition in reversed
-// time.  c is rebuilt from the state that the forward kept for every segment.
+// time.  c is rebuilt from the state that the forward kept for every segment.  330 us for the first shape
+// above, 55 %: ten special-function instructions an element (48 % busy), issue 54 %, and 20 warps on an SM,
+// since a step leaves five values for the second pass.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <initializer_list>
@@ -214,7 +221,7 @@ struct Place {
   }
 };
 
-// The exchange between the threads that share a channel.  `own` is this thread's run; `carry`, the
+// The exchange between the threads that share a channel, one barrier a turn (two in a cluster).  `own` is this thread's run; `carry`, the
 // state entering the tile, becomes the one leaving it.  Returns the state entering this thread's
 // run.  Runs are folded in running order (backward: from the last segment and rank to the first).
 template <int V, bool REVERSE>
@@ -520,7 +527,9 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : kHeld<T, V> ? 5 : 
   if (p.dc0 != nullptr && at.rank == 0 && at.seg == 0) store_state<V>(p.dc0, state_at, carry);
 }
 
-// One step of a batch of streams: a thread takes V channels of one row, nothing is exchanged.
+// One step of a batch of streams: a thread takes V channels of one row, nothing is exchanged.  16 rows of
+// H = 512 bf16 take 1.8 us, a launch; 4096 rows of H = 2048 24 us, 53 % of the measured bandwidth (the general
+// kernel took 53 us, most of it finding its place).
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) scan_step_kernel(const __grid_constant__ ScanArgs p) {
   constexpr bool PRECISE = sizeof(T) == 4;

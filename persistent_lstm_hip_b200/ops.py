@@ -42,6 +42,7 @@ def _first_order(backward):
     return run
 
 
+# autograd's apply() costs about 0.6 us an argument, so what is no tensor goes through it as one.
 # What depends on shapes, strides and types alone (checks, descriptors, sizes) is worked out once for
 # each combination and found again by it in these bounded caches.
 _plan = functools.lru_cache(maxsize=512)
@@ -99,7 +100,8 @@ def _scan_forward(plan, gates, c0, lengths, keep, c_n=None):
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gates, c0, lengths, plan, seq_major):
+    def forward(ctx, gates, c0, how):
+        lengths, plan, seq_major = how
         h, c_n, ckpt = _scan_forward(plan, gates, c0, lengths, True)
         ctx.save_for_backward(gates, lengths, ckpt)
         ctx.seq_major = seq_major
@@ -124,7 +126,7 @@ class _GatedScan(torch.autograd.Function):
             _ptr(dc0), _stream(dev.index))
         if rc:
             _lib.check(rc)
-        return dgates, dc0, None, None, None
+        return dgates, dc0, None
 
 
 def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, *,
@@ -148,7 +150,7 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
             raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
         lengths = lengths.to(device=gates.device, dtype=torch.int32).contiguous()
     if torch.is_grad_enabled() and (gates.requires_grad or (c0 is not None and c0.requires_grad)):
-        return _GatedScan.apply(gates, c0, lengths, plan, seq_major)
+        return _GatedScan.apply(gates, c0, (lengths, plan, seq_major))
     return _scan_forward(plan, gates, c0, lengths, False)[:2]
 
 
@@ -208,7 +210,8 @@ def _dropout(x, drop, residual, dtype):
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, drop, seed):
+    def forward(ctx, x, residual, how):
+        drop, seed = how
         ctx.args = (drop, x.dtype)
         # A tensor seed is kept with its version: changing it before the backward is an error.
         ctx.save_for_backward(seed)
@@ -220,7 +223,7 @@ class _Dropout(torch.autograd.Function):
         drop, dtype = ctx.args
         ctx.saved_tensors
         dx = _dropout(dy.contiguous(), drop, None, dtype) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+        return dx, dy if ctx.needs_input_grad[1] else None, None
 
 
 def _check_residual(residual: torch.Tensor, x: torch.Tensor) -> None:
@@ -248,7 +251,7 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
         _check_residual(residual, x)
     drop = _drop_desc(p, seed, offset, x.device)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, drop, seed if isinstance(seed, torch.Tensor) else None)
+        return _Dropout.apply(x, residual, (drop, seed if isinstance(seed, torch.Tensor) else None))
     return _dropout(x, drop, residual, x.dtype if residual is None else residual.dtype)
 
 
@@ -348,7 +351,9 @@ def _norm_backward(v, weight, stats, dy, dz, eps, drop, x_dtype, w_dtype, need):
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, rows, plan, eps):
+    def forward(ctx, x, weight, bias, how):
+        plan, eps = how
+        rows = _rows(x)
         y, _, stats = _norm_forward(rows, None, weight, bias, plan, None, True)
         ctx.save_for_backward(rows, weight, stats)
         ctx.args = (eps, plan.w_dtype)
@@ -362,13 +367,14 @@ class _LayerNorm(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, _, dw, db = _norm_backward(x, weight, stats, _rows(dy), None, eps, None, x.dtype, w_dtype,
                                        (need[0], False, need[1], need[2]))
-        return dx if dx is None or dy.dim() == 2 else dx.view(dy.shape), dw, db, None, None, None
+        return dx if dx is None or dy.dim() == 2 else dx.view(dy.shape), dw, db, None
 
 
 class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, weight, bias, x2, r2, plan, drop, seed, eps):
-        y, z, stats = _norm_forward(x2, r2, weight, bias, plan, drop, True)
+    def forward(ctx, x, residual, weight, bias, how):
+        plan, drop, seed, eps = how
+        y, z, stats = _norm_forward(_rows(x), _rows(residual), weight, bias, plan, drop, True)
         ctx.save_for_backward(z, weight, stats, seed)
         ctx.args = (drop, eps, x.dtype, plan.w_dtype)
         ctx.set_materialize_grads(False)
@@ -380,7 +386,7 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
         z, weight, stats, _ = ctx.saved_tensors
         drop, eps, x_dtype, w_dtype = ctx.args
         if dy is None and dz is None:
-            return (None,) * 10
+            return (None,) * 5
         shape = (dz if dy is None else dy).shape
         dy = torch.zeros((1, z.shape[1]), dtype=x_dtype, device=z.device).expand(z.shape) if dy is None else _rows(dy)
         dx, dres, dw, db = _norm_backward(z, weight, stats, dy, None if dz is None else _rows(dz), eps, drop, x_dtype,
@@ -388,7 +394,7 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
         if len(shape) != 2:
             dx = None if dx is None else dx.view(shape)
             dres = None if dres is None else dres.view(shape)
-        return dx, dres, dw, db, None, None, None, None, None, None
+        return dx, dres, dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -402,7 +408,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     rows, _, weight, bias, plan = _norm_inputs(x, None, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, rows.detach(), plan, eps)
+        return _LayerNorm.apply(x, weight, bias, (plan, eps))
     y = _norm_forward(rows, None, weight, bias, plan, None, False)[0]
     return y if x.dim() == 2 else y.view(x.shape)
 
@@ -425,7 +431,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
                                     (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
-        return _DropoutAddLayerNorm.apply(x, residual, weight, bias, x2.detach(), r2.detach(), plan, drop,
-                                          seed if isinstance(seed, torch.Tensor) else None, eps)
+        return _DropoutAddLayerNorm.apply(x, residual, weight, bias,
+                                          (plan, drop, seed if isinstance(seed, torch.Tensor) else None, eps))
     y, z, _ = _norm_forward(x2, r2, weight, bias, plan, drop, False)
     return (y, z) if x.dim() == 2 else (y.view(x.shape), z.view(x.shape))

@@ -590,10 +590,11 @@ int64_t backward_ctas(const plstm_norm_desc& d, const Split& s, int per_sm) {
 constexpr int kBackwardThreads = 1024;  // per SM, the most that the workspace provides for
 int backward_most(const Split& s) { return std::max(1, kBackwardThreads / s.block()); }
 
-// CTAs of a kernel that an SM holds, remembered for the last block and shared-memory size asked for.
+// CTAs of a kernel that an SM holds, remembered for the last device, block and shared-memory size asked
+// for; on a miss the kernel is also allowed that much shared memory on the current device.
 template <typename Kernel>
-int32_t resident(Kernel kernel, std::atomic<uint64_t>& memo, int block, size_t smem, int* per_sm) {
-  const uint64_t key = (uint64_t)block << 40 | (uint64_t)smem << 8, seen = memo.load(std::memory_order_relaxed);
+int32_t resident(Kernel kernel, std::atomic<uint64_t>& memo, int device, int block, size_t smem, int* per_sm) {
+  const uint64_t key = (uint64_t)device << 52 | (uint64_t)block << 40 | (uint64_t)smem << 8, seen = memo.load(std::memory_order_relaxed);
   if ((seen & ~(uint64_t)255) == key && (seen & 255) != 0) {
     *per_sm = (int)(seen & 255);
     return PLSTM_OK;
@@ -610,7 +611,7 @@ template <bool BACKWARD, typename Kernel>
 int32_t launch(Kernel kernel, std::atomic<uint64_t>& memo, const plstm_norm_desc& d, const NormArgs& a, const Split& s,
                size_t smem, int* grid, cudaStream_t st) {
   int per_sm = 0;
-  if (const int32_t rc = resident(kernel, memo, s.block(), smem, &per_sm)) return rc;
+  if (const int32_t rc = resident(kernel, memo, d.device, s.block(), smem, &per_sm)) return rc;
   *grid = (int)(BACKWARD ? backward_ctas(d, s, std::min(per_sm, backward_most(s))) : forward_ctas(d, s, per_sm));
   kernel<<<*grid, s.block(), smem, st>>>(a);
   PLSTM_TRY_CUDA(cudaGetLastError());

@@ -84,11 +84,10 @@ def _scan_plan(shape, strides, dtype, index, seq_major, dh_strides=None) -> _Sca
     return _ScanPlan(_byref(d), (shape[b], H), h, nbytes.value // 4, d)
 
 
-def _scan_forward(plan, gates, c0, lengths, keep, c_n=None):
+def _scan_forward(plan, gates, c0, lengths, keep):
     dev = gates.device
     h = _empty(plan.h, dtype=gates.dtype, device=dev)
-    if c_n is None:
-        c_n = _empty(plan.state, dtype=_F32, device=dev)
+    c_n = _empty(plan.state, dtype=_F32, device=dev)
     ckpt = _empty(plan.checkpoints, dtype=_F32, device=dev) if keep else None
     rc = _lib.load().plstm_gated_scan_forward(
         plan.desc, gates.data_ptr(), _ptr(lengths), _ptr(c0), h.data_ptr(), c_n.data_ptr(), _ptr(ckpt),
@@ -169,18 +168,24 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
                              "no_grad")
         h, c_n = gated_scan(gates[:, None], c)
         return h[:, 0], c_n
-    # One step of [1, B, 4H], so that h comes out as [1, B, H] without a view of the gates.
-    shape, strides = gates.shape, gates.stride()
-    plan = _scan_plan((1, *shape), (0, *strides), gates.dtype, gates.device.index, True)
-    c = _require_cuda(c, "c", gates.device, _F32)
+    # One step of [1, B, 4H]; h is allocated without the axis of one.
+    dev = gates.device
+    plan = _scan_plan((1, *gates.shape), (0, *gates.stride()), gates.dtype, dev.index, True)
+    c = _require_cuda(c, "c", dev, _F32)
     if c.shape != plan.state:
         raise ValueError(f"c must be {list(plan.state)}, got {tuple(c.shape)}")
-    if out_c is not None:
-        _require_cuda(out_c, "out_c", gates.device, _F32)
+    if out_c is None:
+        out_c = _empty(plan.state, dtype=_F32, device=dev)
+    else:
+        _require_cuda(out_c, "out_c", dev, _F32)
         if out_c.shape != plan.state or not out_c.is_contiguous():
             raise ValueError(f"out_c must be {list(plan.state)} and contiguous")
-    h, c_n, _ = _scan_forward(plan, gates, c, None, False, out_c)
-    return h[0], c_n
+    h = _empty(plan.state, dtype=gates.dtype, device=dev)
+    rc = _lib.load().plstm_gated_scan_forward(plan.desc, gates.data_ptr(), None, c.data_ptr(), h.data_ptr(),
+                                              out_c.data_ptr(), None, _stream(dev.index))
+    if rc:
+        _lib.check(rc)
+    return h, out_c
 
 
 # ---- dropout --------------------------------------------------------------------------------

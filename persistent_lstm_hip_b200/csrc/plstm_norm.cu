@@ -10,9 +10,9 @@
 //
 // Both directions are bound by instruction issue before memory.  Measured at 65536 x 1024 bf16 with f32
 // weights: forward 53 us, 78 % of the measured 6.54 TB/s (14 instructions an element); backward with the
-// weight gradients 86 us, 71 % (27 an element).  With residual and dropout at 131072 x 512: 126 and 161 us, 65 %
-// and 64 % (Philox adds 11.5 an element); with f32 throughout at 65536 x 512: 88 and 113 us, 93 % and 91 %.
-// Rows 1001 wide (33000 of them): 57 and 108 us against 27 and 44 us that their bytes would take at the 1024's rate:
+// weight gradients 86 us, 71 % (27 an element).  With residual and dropout at 131072 x 512: 127 and 158 us, 65 %
+// and 65 % (Philox adds 11.5 an element); with f32 throughout at 65536 x 512: 88 and 113 us, 93 % and 91 %.
+// Rows 1001 wide (33000 of them): 57 and 91 us against 26 and 42 us that their bytes would take at the 1024's rate:
 // the masked ends and the columns' places cost instructions.
 #include <algorithm>
 #include <atomic>
@@ -321,11 +321,17 @@ __global__ void __launch_bounds__(max_block(CH), CH == 4 ? 1 : 2) norm_forward_k
   }
 }
 
+// 128 registers let four CTAs of 128 threads share an SM.  Two chunks of 16-bit v fit (33000 x 1001 bf16 91 us
+// against 107 us with 168 registers; fused 158 us against 170 us; fused 8192 x 4096 97 us against 119 us), two of
+// f32 do not (fused 65536 x 512: 113 us with 168, 176 us with 128; under f16 x 98 us and 128 us).  Four chunks go
+// up to CTAs of 544 threads.
+constexpr int backward_registers(int ch, int size) { return ch == 4 ? 96 : ch == 1 ? 112 : size == 2 ? 128 : 168; }
+
 // TV: the normalised tensor's type (x or z).  partial [gridDim.x][2][cols], or NULL.  A team's rows
 // all have one phase (their distance is a multiple of 8), so a thread's columns stay its own and
 // the sums of the weight gradients stay with it: in registers, or (CH = 4) in shared memory.
 template <typename TX, typename TV, int CH, bool FUSED, bool WHOLE>
-__global__ void __launch_bounds__(max_block(CH), CH == 1 ? 2 : 1) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __maxnreg__(backward_registers(CH, sizeof(TV))) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr bool REGS = CH < 4;
   __shared__ float scratch[2 * 2 * 32 * (kTeamBlock / 32)];
   extern __shared__ __align__(16) float columns[];

@@ -203,14 +203,10 @@ __device__ __forceinline__ uint64_t uniform_seed(const Drop& d) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// x / (1 - p) where the word keeps the element, else 0 (whatever x is).  The explicit
-// rounding keeps the compiler from contracting the product with a later sum, so that the
-// fused and the separate calls give the same bits.
-__device__ __forceinline__ float drop_one(const Drop& d, uint32_t word, float x) {
-  return word >= d.threshold ? __fmul_rn(x, d.scale) : 0.0f;
-}
-
-// Applies the dropout to the eight elements of the Philox blocks (lo, hi) and (lo + 1, hi); lo is even.
+// Applies the dropout to the eight elements of the Philox blocks (lo, hi) and (lo + 1, hi), lo even:
+// x / (1 - p) where the word keeps the element, else 0 (whatever x is).  The products are instructions of
+// their own (f32x2, each rounded), never contracted with a later sum, so that the fused and the separate
+// calls give the same bits.
 __device__ __forceinline__ void drop_eight(const Drop& d, uint64_t seed, uint32_t lo, uint32_t hi, float (&x)[8]) {
   if (d.mode == 0) return;
   if (d.mode == 2) {
@@ -221,10 +217,12 @@ __device__ __forceinline__ void drop_eight(const Drop& d, uint64_t seed, uint32_
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const uint4 w = philox(lo + q, hi, d.offset, seed);
-    x[4 * q] = drop_one(d, w.x, x[4 * q]);
-    x[4 * q + 1] = drop_one(d, w.y, x[4 * q + 1]);
-    x[4 * q + 2] = drop_one(d, w.z, x[4 * q + 2]);
-    x[4 * q + 3] = drop_one(d, w.w, x[4 * q + 3]);
+    const F<2> a = F<2>::of(x[4 * q], x[4 * q + 1]) * F<2>::of(d.scale);
+    const F<2> b = F<2>::of(x[4 * q + 2], x[4 * q + 3]) * F<2>::of(d.scale);
+    x[4 * q] = w.x >= d.threshold ? a.x : 0.0f;
+    x[4 * q + 1] = w.y >= d.threshold ? a.y : 0.0f;
+    x[4 * q + 2] = w.z >= d.threshold ? b.x : 0.0f;
+    x[4 * q + 3] = w.w >= d.threshold ? b.y : 0.0f;
   }
 }
 

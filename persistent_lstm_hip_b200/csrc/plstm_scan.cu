@@ -40,14 +40,14 @@ namespace {
 constexpr int kSeg = PLSTM_SCAN_SEGMENT;
 constexpr int kMaxThreads = 128;
 constexpr int kMaxCluster = 16;
-constexpr int kWanted = 384;  // CTAs of 128 threads that fill the GPU: 2.6 on an SM
-constexpr int kAlone = 16 * kSMs;  // warps that do
+constexpr int kWanted = 384;       // CTAs that keep the GPU busy (make_plan)
+constexpr int kAlone = 16 * kSMs;  // warps that do without splitting time
 
 struct ScanArgs {
   int B, T, H;
-  int cl, seg, groups; // channel lanes, time segments and channel groups of a CTA (their product: threads)
-  int ch_blocks;      // CTAs (or clusters) along the channels of a row
-  int stage_at;       // where the staged gates begin in shared memory
+  int cl, seg, groups;  // channel lanes, time segments and channel groups of a CTA (their product: threads)
+  int ch_blocks;        // groups along the channels of a row
+  int stage_at;         // where shared memory past the exchange begins
   int64_t g_sb, g_st, h_sb, h_st, d_sb, d_st;
   const void* gates;
   const int32_t* lengths;
@@ -221,16 +221,18 @@ struct Place {
   }
 };
 
-// The exchange between the threads that share a channel, one barrier a turn (two in a cluster).  `own` is this thread's run; `carry`, the
-// state entering the tile, becomes the one leaving it.  Returns the state entering this thread's
-// run.  Runs are folded in running order (backward: from the last segment and rank to the first).
+// The exchange between the threads that share a channel, one barrier a turn (two in a cluster).  `own`
+// is this thread's run; `carry`, the state entering the tile, becomes the one leaving it.  Returns the
+// state entering this thread's run.  Runs are folded in running order (backward: from the last segment
+// and rank to the first).  The buffers alternate from turn to turn, so a turn's barrier also frees the
+// turn before's.
 template <int V, bool REVERSE>
 struct Exchange {
   Run<V>* segs;   // [2][seg][cl] of the group
   Run<V>* ranks;  // [2][kMaxCluster][cl]
 
   __device__ __forceinline__ F<V> operator()(const ScanArgs& p, const Place<V>& at, int turn, const Run<V>& own,
-                                                 F<V>& carry) const {
+                                             F<V>& carry) const {
     const int parity = turn & 1;
     Run<V>* const mine = segs + parity * p.seg * p.cl + at.cl;
     const int order = REVERSE ? p.seg - 1 - at.seg : at.seg;
@@ -579,11 +581,19 @@ __global__ void __launch_bounds__(kMaxThreads) scan_step_kernel(const __grid_con
   }
 }
 
-// How the work is split.  A CTA has 128 threads of up to 128 registers (four on an SM): 32 channel
-// lanes (128 bytes of a 16-bit row) by four segments.  Where that gives fewer than 512 CTAs, a CTA takes
-// fewer channels and more segments, down to rows of 32 bytes, and then the CTAs of a cluster share a
-// channel; there are never more segments than the sequence has.  Where there are warps enough without
-// splitting time, every warp walks its row alone.
+// How the work is split (B x T x H; GPU times).  A CTA has 128 threads of up to 128 registers, four or five
+// on an SM: 32 channel lanes, 128 bytes of a 16-bit row, by four segments of time.
+// - Fewer than kWanted CTAs: fewer channels and more segments each, down to rows of 32 bytes (8 x 4096 x 1024
+//   bf16 forward: 111 us with rows of 32 bytes, 116 us with clusters of four), or of 64 where rows do not
+//   start on sectors (16 x 2000 x 310: 50 us with 64, 63 us with 32); then the CTAs of a cluster share a
+//   channel (1 x 65536 x 512: 178 us with 16, 234 us with 8), and with 16 of them still too few, rows of 16
+//   bytes (1 x 40759 x 21 f16, forward and backward: 77 us, without 419 us).
+// - The backward of 16-bit pairs starts from 16 lanes by eight segments, shorter CTAs that fill its five
+//   places more evenly (512 x 1000 x 128 f16: 332 us, with 32 lanes 371 us).
+// - kAlone warps or more without splitting time: every warp walks its rows alone (4096 x 64 x 128 bf16: forward
+//   79 us against 93 us, backward 142 us against 156 us); with 1024 warps splitting wins (512 x 1000 x 128 f16
+//   forward: 171 us with four segments, 193 us with two).
+// There are never more segments than the sequence has, and a CTA that they do not fill takes several groups.
 struct Plan {
   int cl, seg, groups, cluster, ch_blocks;
 };
@@ -675,7 +685,8 @@ int32_t launch_step(const ScanArgs& a, cudaStream_t s) {
   return PLSTM_OK;
 }
 
-// A single step, or up to four, would waste most of a segment of eight.
+// A single step, or up to four, would waste most of a segment of eight (forward and backward of
+// 4096 x 3 x 512 bf16: 32 + 47 us against 51 + 75 us; backward of 4096 x 1 x 2048: 78 us against 276 us).
 template <typename T, int V>
 int32_t dispatch_steps(bool backward, int dtype, const ScanArgs& a, cudaStream_t s) {
   if (backward && a.T == 1) return launch<T, V, 1, false>(true, a, s);

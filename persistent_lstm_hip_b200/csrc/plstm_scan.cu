@@ -22,9 +22,9 @@
 //
 // Backward, with e_t = dh_t o_t (1 - tanh(c_t)^2): dc_t = e_t + G_t, G_{t-1} = f_t dc_t, where
 // G enters the last step as dc_n and leaves the first as dc0: the same composition in reversed
-// time.  c is rebuilt from the state that the forward kept for every segment.  330 us for the first shape
-// above, 55 %: ten special-function instructions an element (48 % busy), issue 54 %, and 20 warps on an SM,
-// since a step leaves five values for the second pass.
+// time.  c is rebuilt from the state that the forward kept for every segment.  298 us for the first shape
+// above, 61 %: ten special-function instructions an element and 16 warps on an SM, since a step leaves
+// five values for the second pass.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <initializer_list>
@@ -431,14 +431,15 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : STAGED ? 5 : 4) sc
   if (at.rank == 0 && at.seg == 0) store_state<V>(p.c_n, state_at, carry);
 }
 
-// Two of the five values that a step keeps for the second pass wait in shared memory, where the registers
-// then leave room for a fifth CTA on an SM: one row of 65,536 steps, H = 512, bf16 takes 283 us against 396 us,
-// 64 x 1000 x 310 takes 120 us against 155 us.  Not for pairs of f32 channels, whose loads alone fill the
-// registers of five CTAs (64 x 2000 x 256: 251 us without, 328 us with).
+// Two of the five values that a step keeps for the second pass wait in shared memory (not for pairs of f32
+// channels: 64 x 2000 x 256 251 us without, 328 us with).  For pairs of 16-bit channels this frees the
+// registers of four CTAs an SM from spills (512 x 1000 x 128 f16: 298 us, without 336 us), or makes room for a
+// fifth, which only the long turns of a cluster repay (CTAS = 5: one row of 65,536 steps, H = 512, bf16, 287 us
+// against 357 us with four; 512 x 1000 x 128 330 us).
 template <typename T, int V>
 constexpr bool kHeld = V * sizeof(T) <= 4;
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : kHeld<T, V> ? 5 : 4) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
+template <typename T, int V, int K, int CTAS>
+__global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : CTAS) scan_backward_kernel(const __grid_constant__ ScanArgs p, int cluster) {
   constexpr bool PRECISE = sizeof(T) == 4, ONE = K < kSeg, HELD = kHeld<T, V> && !ONE;  // ONE: one segment is the whole sequence
   extern __shared__ __align__(16) unsigned char smem[];
   const Place<V> at(p, cluster);
@@ -588,8 +589,6 @@ __global__ void __launch_bounds__(kMaxThreads) scan_step_kernel(const __grid_con
 //   start on sectors (16 x 2000 x 310: 50 us with 64, 63 us with 32); then the CTAs of a cluster share a
 //   channel (1 x 65536 x 512: 178 us with 16, 234 us with 8), and with 16 of them still too few, rows of 16
 //   bytes (1 x 40759 x 21 f16, forward and backward: 77 us, without 419 us).
-// - The backward of 16-bit pairs starts from 16 lanes by eight segments, shorter CTAs that fill its five
-//   places more evenly (512 x 1000 x 128 f16: 332 us, with 32 lanes 371 us).
 // - kAlone warps or more without splitting time: every warp walks its rows alone (4096 x 64 x 128 bf16: forward
 //   79 us against 93 us, backward 142 us against 156 us); with 1024 warps splitting wins (512 x 1000 x 128 f16
 //   forward: 171 us with four segments, 193 us with two).
@@ -598,17 +597,16 @@ struct Plan {
   int cl, seg, groups, cluster, ch_blocks;
 };
 
-Plan make_plan(int B, int T, int H, int V, int K, int size, bool backward) {
+Plan make_plan(int B, int T, int H, int V, int K, int size) {
   Plan p;
   const int lanes = (H + V - 1) / V, segments = std::max(1, (T + K - 1) / K);
   p.cl = 1;
   const int narrowest = (int64_t)H * size % 32 == 0 ? 32 : 64;  // bytes of a row that cost whole sectors
-  const int widest = backward && segments >= 8 && narrowest == 32 && V * size <= 4 ? 16 : 32;
-  while (p.cl < widest && p.cl < lanes) p.cl *= 2;
+  while (p.cl < 32 && p.cl < lanes) p.cl *= 2;
   const auto blocks = [&] { return (int64_t)B * ((lanes + p.cl - 1) / p.cl); };
   while (p.cl * V * size / 2 >= narrowest && blocks() < kWanted && kMaxThreads / p.cl < segments) p.cl /= 2;
   p.seg = 1;
-  if (blocks() * p.cl < 32 * kAlone || p.cl < 16)
+  if (blocks() < kAlone || p.cl < 32)
     while (p.seg * p.cl < kMaxThreads && p.seg < segments) p.seg *= 2;
   p.cluster = 1;
   while (p.cluster < kMaxCluster && blocks() * p.cluster < kWanted && p.seg * p.cluster < segments) p.cluster *= 2;
@@ -625,7 +623,7 @@ Plan make_plan(int B, int T, int H, int V, int K, int size, bool backward) {
 // STAGED: V channels of a lane that come through shared memory, 16 bytes a copy.
 template <typename T, int V, int K, bool STAGED>
 int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
-  const Plan plan = make_plan(a.B, a.T, a.H, V, K, (int)sizeof(T), backward);
+  const Plan plan = make_plan(a.B, a.T, a.H, V, K, (int)sizeof(T));
   a.cl = plan.cl;
   a.seg = plan.seg;
   a.groups = plan.groups;
@@ -660,7 +658,12 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
     note_launches(1);
     return PLSTM_OK;
   };
-  if (backward) return go(scan_backward_kernel<T, V, K>);
+  if (backward) {
+    if constexpr (K == kSeg && V == 2 && sizeof(T) == 2) {
+      if (plan.cluster > 1) return go(scan_backward_kernel<T, V, K, 5>);
+    }
+    return go(scan_backward_kernel<T, V, K, V == 1 ? 5 : 4>);
+  }
   if constexpr (STAGED) {
     if (staged) return go(scan_forward_kernel<T, V, K, true>);
   }

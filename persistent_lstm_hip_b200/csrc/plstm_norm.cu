@@ -597,7 +597,9 @@ constexpr int kBackwardThreads = 1024;  // per SM, the most that the workspace p
 int backward_most(const Split& s) { return std::max(1, kBackwardThreads / s.block()); }
 
 // CTAs of a kernel that an SM holds, remembered for the last device, block and shared-memory size asked
-// for; on a miss the kernel is also allowed that much shared memory on the current device.
+// for; on a miss the kernel is also allowed all the shared memory that any shape needs (one value, so
+// that threads launching different shapes do not take it back from one another).
+constexpr int kMostShared = 216 * 1024;  // with the kernels' own 2 KB and the system's 1 KB below 227 KB
 template <typename Kernel>
 int32_t resident(Kernel kernel, std::atomic<uint64_t>& memo, int device, int block, size_t smem, int* per_sm) {
   const uint64_t key = (uint64_t)device << 52 | (uint64_t)block << 40 | (uint64_t)smem << 8, seen = memo.load(std::memory_order_relaxed);
@@ -606,7 +608,7 @@ int32_t resident(Kernel kernel, std::atomic<uint64_t>& memo, int device, int blo
     return PLSTM_OK;
   }
   if (smem > 40 * 1024)
-    PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
   PLSTM_TRY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kernel, block, smem));
   *per_sm = std::max(1, *per_sm);
   memo.store(key | (uint64_t)*per_sm, std::memory_order_relaxed);

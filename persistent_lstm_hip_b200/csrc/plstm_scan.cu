@@ -652,8 +652,7 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
     if (plan.cluster > 8)  // beyond the portable size: has to be allowed for the kernel
       PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (cfg.dynamicSmemBytes > 48 * 1024)
-      PLSTM_TRY_CUDA(
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
+      PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
     PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan.cluster));
     note_launches(1);
     return PLSTM_OK;

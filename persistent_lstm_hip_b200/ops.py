@@ -203,6 +203,12 @@ def _drop_desc(p: float, seed: Union[int, torch.Tensor], offset: int, device: to
     return _lib.DropoutDesc(p, seed, offset, None)
 
 
+def _saved_drop(drop, seed):
+    """The forward's descriptor for its backward.  A tensor seed is read where autograd holds it: saved-tensor
+    hooks (checkpointing, offloading) keep a copy, and the forward's own tensor may be changed or freed by then."""
+    return drop if seed is None else _lib.DropoutDesc(drop.p, 0, drop.offset, seed.data_ptr())
+
+
 def _dropout(x, drop, residual, dtype):
     dev = x.device
     y = _empty(x.shape, dtype=dtype, device=dev)
@@ -226,8 +232,8 @@ class _Dropout(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         drop, dtype = ctx.args
-        ctx.saved_tensors
-        dx = _dropout(dy.contiguous(), drop, None, dtype) if ctx.needs_input_grad[0] else None
+        (seed,) = ctx.saved_tensors
+        dx = _dropout(dy.contiguous(), _saved_drop(drop, seed), None, dtype) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None
 
 
@@ -388,14 +394,14 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, dy, dz):
-        z, weight, stats, _ = ctx.saved_tensors
+        z, weight, stats, seed = ctx.saved_tensors
         drop, eps, x_dtype, w_dtype = ctx.args
         if dy is None and dz is None:
             return (None,) * 5
         shape = (dz if dy is None else dy).shape
         dy = torch.zeros((1, z.shape[1]), dtype=x_dtype, device=z.device).expand(z.shape) if dy is None else _rows(dy)
-        dx, dres, dw, db = _norm_backward(z, weight, stats, dy, None if dz is None else _rows(dz), eps, drop, x_dtype,
-                                          w_dtype, ctx.needs_input_grad)
+        dx, dres, dw, db = _norm_backward(z, weight, stats, dy, None if dz is None else _rows(dz), eps,
+                                          _saved_drop(drop, seed), x_dtype, w_dtype, ctx.needs_input_grad)
         if len(shape) != 2:
             dx = None if dx is None else dx.view(shape)
             dres = None if dres is None else dres.view(shape)

@@ -1,0 +1,49 @@
+"""The training and streaming operators' calls on the GPU: what autograd, hooks, tracers and threads
+see of them."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import operator_forms as forms
+import persistent_lstm_hip_b200 as plstm
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _randn(*shape, dtype=F32, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed + 31 * len(shape))).to("cuda:0", dtype)
+
+
+# ---- a tensor seed under saved-tensor hooks ----------------------------------------------------------
+@pytest.mark.parametrize("fused", [False, True])
+def test_temporary_seed_under_a_checkpoint(cuda_device, fused):
+    """The seed is made inside the checkpointed function and freed before the backward: the mask of
+    the gradients is the forward's all the same."""
+    n, p = 4096, 0.5
+    base = torch.tensor([41], device=cuda_device)
+
+    def call(x):
+        if fused:
+            return plstm.dropout_add_layer_norm(x, torch.zeros_like(x), None, None, p, base + 1)[1]
+        return plstm.dropout(x, p, base + 1)
+
+    x = _randn(8, n // 8).requires_grad_(True)
+    y = checkpoint(call, x, use_reentrant=False)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(x))
+    keep = forms.keep_mask(np.arange(n), p, 42, 0).view(8, n // 8)
+    assert torch.equal(y.detach().cpu() != 0, keep)
+    assert torch.equal(dx.cpu(), keep.float() * 2)
+
+
+def test_seed_advanced_under_hooks_that_copy(cuda_device):
+    x, seed = _randn(1000).requires_grad_(True), torch.tensor([42], device=cuda_device)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t):
+        y = plstm.dropout(x, 0.5, seed)
+    seed.add_(1)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(x))
+    assert torch.equal(dx.cpu(), forms.keep_mask(np.arange(1000), 0.5, 42, 0).float() * 2)

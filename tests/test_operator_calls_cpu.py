@@ -1,0 +1,86 @@
+"""What the Python calls of the training and streaming operators hand to the library and to
+autograd, on the CPU: a stand-in takes the library's place and reads the pointers it is given."""
+from __future__ import annotations
+
+import ctypes
+import types
+
+import pytest
+import torch
+
+from persistent_lstm_hip_b200 import _lib, ops
+
+
+class StandIn:
+    """Calls of the C ABI that note what they were given.  Dropout writes its seed into every element."""
+
+    def __init__(self):
+        self.seeds = []
+
+    def plstm_dropout(self, drop, n, x, x_dtype, residual, y, y_dtype, device, stream):
+        self.seeds.append(self._seed(drop))
+        (ctypes.c_float * n).from_address(y)[:] = [float(self.seeds[-1])] * n
+        return 0
+
+    def plstm_layer_norm_forward(self, desc, drop, *rest):
+        self.seeds.append(None if drop is None else self._seed(drop))
+        return 0
+
+    def plstm_layer_norm_backward_workspace_size(self, desc, nbytes):
+        nbytes._obj.value = 256
+        return 0
+
+    def plstm_layer_norm_backward(self, desc, drop, *rest):
+        self.seeds.append(None if drop is None else self._seed(drop))
+        return 0
+
+    @staticmethod
+    def _seed(drop):
+        d = drop._obj
+        return ctypes.c_uint64.from_address(d.seed_ptr).value if d.seed_ptr else d.seed
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    lib = StandIn()
+    # A CPU tensor's device has no index.
+    numbered = lambda kind: lambda *fields: kind(*(0 if f is None else f for f in fields))
+    monkeypatch.setattr(ops, "_lib", types.SimpleNamespace(
+        load=lambda: lib, check=_lib.check, DropoutDesc=_lib.DropoutDesc, NormDesc=numbered(_lib.NormDesc),
+        ScanDesc=numbered(_lib.ScanDesc), NORM_MAX_COLS=_lib.NORM_MAX_COLS))
+    monkeypatch.setattr(ops, "_stream", lambda index: 0)
+    monkeypatch.setattr(ops, "_cuda_float", lambda t, name: t if t.stride(-1) == 1 else t.contiguous())
+    monkeypatch.setattr(ops, "_require_cuda", lambda t, name, device, dtype=None: t.contiguous())
+    return lib
+
+
+# ---- a tensor seed under saved-tensor hooks ----------------------------------------------------------
+def _copies():
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t)
+
+
+def test_dropout_backward_reads_the_seed_that_autograd_kept(stand_in):
+    """Hooks that pack a copy: autograd neither holds the caller's seed nor watches its version."""
+    x, seed = torch.zeros(8, requires_grad=True), torch.tensor([42])
+    with _copies():
+        y = ops.dropout(x, 0.5, seed)
+    seed.add_(1)
+    (dx,) = torch.autograd.grad(y, x, torch.ones(8))
+    assert stand_in.seeds == [42, 42] and (dx == 42).all()
+
+
+def test_fused_backward_reads_the_seed_that_autograd_kept(stand_in):
+    x, res, seed = torch.zeros(2, 8, requires_grad=True), torch.zeros(2, 8), torch.tensor([42])
+    with _copies():
+        y, z = ops.dropout_add_layer_norm(x, res, None, None, 0.5, seed)
+    seed.add_(1)
+    torch.autograd.grad(y, x, torch.ones(2, 8))
+    assert stand_in.seeds == [42, 42]
+
+
+def test_an_int_seed_is_the_backwards_too(stand_in):
+    x = torch.zeros(8, requires_grad=True)
+    with _copies():
+        y = ops.dropout(x, 0.5, 7)
+    torch.autograd.grad(y, x, torch.ones(8))
+    assert stand_in.seeds == [7, 7]

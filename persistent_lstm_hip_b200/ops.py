@@ -128,13 +128,25 @@ class _GatedScan(torch.autograd.Function):
         return dgates, dc0, None
 
 
+def _fit_lengths(lengths: torch.Tensor, top: int) -> torch.Tensor:
+    """`lengths` within int32.  The kernel clamps to [0, top]; what int32 cannot hold is clamped before it would wrap."""
+    if lengths.dtype is torch.uint64:  # the upper half is negative as int64
+        lengths = lengths.to(torch.int64)
+        lengths = torch.where(lengths < 0, top, lengths)
+    elif lengths.dtype is torch.uint32:
+        lengths = lengths.to(torch.int64)
+    if lengths.dtype is torch.int64:
+        lengths = lengths.clamp(0, top)
+    return lengths
+
+
 def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, *,
                seq_major: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """Gate projections -> (h, c_n) of an LSTM layer whose gates do not look back.
 
     gates [B,T,4H] (or [T,B,4H] with seq_major=True) holds the pre-activations in nn.LSTM's gate
     order i, f, g, o:  c_t = sigmoid(f) c_{t-1} + sigmoid(i) tanh(g),  h_t = sigmoid(o) tanh(c_t).
-    c0 [B,H] f32 (default zeros); lengths [B]: the state stands still from a row's length on, h is
+    c0 [B,H] f32 (default zeros); lengths [B], clamped to [0, T]: the state stands still from a row's length on, h is
     zero there, and neither the gates nor their gradient count.  Returns h in the gates' type and
     layout and c_n [B,H] f32.  Differentiable in gates and c0.
     """
@@ -147,7 +159,8 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.shape != plan.state[:1]:
             raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
-        lengths = lengths.to(device=gates.device, dtype=torch.int32).contiguous()
+        top = gates.shape[0 if seq_major else 1]
+        lengths = _fit_lengths(lengths, top).to(device=gates.device, dtype=torch.int32).contiguous()
     if torch.is_grad_enabled() and (gates.requires_grad or (c0 is not None and c0.requires_grad)):
         return _GatedScan.apply(gates, c0, (lengths, plan, seq_major))
     return _scan_forward(plan, gates, c0, lengths, False)[:2]

@@ -47,3 +47,23 @@ def test_seed_advanced_under_hooks_that_copy(cuda_device):
     seed.add_(1)
     (dx,) = torch.autograd.grad(y, x, torch.ones_like(x))
     assert torch.equal(dx.cpu(), forms.keep_mask(np.arange(1000), 0.5, 42, 0).float() * 2)
+
+
+# ---- lengths --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", ["cuda:0", "cpu"])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16,
+                                   torch.uint32, torch.uint64, torch.bool])
+def test_lengths_of_any_type_are_clamped_not_wrapped(cuda_device, dtype, dev):
+    B, T, H = 4, 300, 8
+    top = 1 if dtype is torch.bool else torch.iinfo(dtype).max
+    values = [0, 1, top, min(top, 2 ** 32 + 5)]
+    gates, c0 = _randn(B, T, 4 * H), _randn(B, H)
+    want = plstm.gated_scan(gates, c0, torch.tensor([min(v, T) for v in values], dtype=torch.int32))
+    got = plstm.gated_scan(gates, c0, torch.tensor(values, dtype=dtype).to(dev))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_lengths_below_int32_are_zero(cuda_device):
+    gates, c0 = _randn(2, 9, 16), _randn(2, 4)
+    h, c_n = plstm.gated_scan(gates, c0, torch.tensor([-(2 ** 31) - 7, torch.iinfo(torch.int64).min]))
+    assert (h == 0).all() and torch.equal(c_n, c0)

@@ -15,7 +15,16 @@ class StandIn:
     """Calls of the C ABI that note what they were given.  Dropout writes its seed into every element."""
 
     def __init__(self):
-        self.seeds = []
+        self.seeds, self.lengths = [], []
+
+    def plstm_gated_scan_checkpoint_size(self, desc, nbytes):
+        nbytes._obj.value = 4096
+        return 0
+
+    def plstm_gated_scan_forward(self, desc, gates, lengths, c0, h, c_n, checkpoints, stream):
+        if lengths:
+            self.lengths.append(list((ctypes.c_int32 * desc._obj.batch).from_address(lengths)))
+        return 0
 
     def plstm_dropout(self, drop, n, x, x_dtype, residual, y, y_dtype, device, stream):
         self.seeds.append(self._seed(drop))
@@ -84,3 +93,23 @@ def test_an_int_seed_is_the_backwards_too(stand_in):
         y = ops.dropout(x, 0.5, 7)
     torch.autograd.grad(y, x, torch.ones(8))
     assert stand_in.seeds == [7, 7]
+
+
+# ---- lengths --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("seq_major", [False, True])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16,
+                                   torch.uint32, torch.uint64])
+def test_lengths_of_any_type_are_clamped_not_wrapped(stand_in, dtype, seq_major):
+    B, T = 4, 300
+    top = torch.iinfo(dtype).max
+    values = [0, 7, top, min(top, 2 ** 32 + 5)]
+    ops.gated_scan(torch.zeros((T, B, 8) if seq_major else (B, T, 8)), lengths=torch.tensor(values, dtype=dtype),
+                   seq_major=seq_major)
+    # The kernel's own clamp completes what fits into int32.
+    assert [min(max(v, 0), T) for v in stand_in.lengths[0]] == [min(v, T) for v in values]
+
+
+def test_negative_lengths_are_zero(stand_in):
+    values = [-1, -(2 ** 31) - 7, torch.iinfo(torch.int64).min]
+    ops.gated_scan(torch.zeros(3, 5, 8), lengths=torch.tensor(values))
+    assert all(v <= 0 for v in stand_in.lengths[0])

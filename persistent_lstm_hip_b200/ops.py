@@ -193,6 +193,8 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
         _require_cuda(out_c, "out_c", dev, _F32)
         if out_c.shape != plan.state or not out_c.is_contiguous():
             raise ValueError(f"out_c must be {list(plan.state)} and contiguous")
+        # The kernel writes behind autograd's back: a graph that saved this state has to notice.
+        torch.autograd.graph.increment_version(out_c)
     h = _empty(plan.state, dtype=gates.dtype, device=dev)
     rc = _lib.load().plstm_gated_scan_forward(plan.desc, gates.data_ptr(), None, c.data_ptr(), h.data_ptr(),
                                               out_c.data_ptr(), None, _stream(dev.index))

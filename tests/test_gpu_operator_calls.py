@@ -67,3 +67,29 @@ def test_lengths_below_int32_are_zero(cuda_device):
     gates, c0 = _randn(2, 9, 16), _randn(2, 4)
     h, c_n = plstm.gated_scan(gates, c0, torch.tensor([-(2 ** 31) - 7, torch.iinfo(torch.int64).min]))
     assert (h == 0).all() and torch.equal(c_n, c0)
+
+
+# ---- writes into the caller's state --------------------------------------------------------------------
+def test_streaming_from_a_state_whose_graph_is_still_needed(cuda_device):
+    """The regressor's states are attached to its graph; streaming on from them in place and then
+    differentiating is an error, never a gradient with the new values."""
+    torch.manual_seed(0)
+    m = plstm.GatedScanRegressor(3, 16, 2, 2).to(cuda_device)
+    _, state = m(_randn(2, 7, 3))
+    loss = (state[0] ** 2).sum()
+    m.step(_randn(2, 3), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    _, state = m(_randn(2, 7, 3))
+    loss = (state[0] ** 2).sum()
+    m.step(_randn(2, 3), [c.detach().clone() for c in state])
+    loss.backward()
+
+
+def test_step_in_inference_mode(cuda_device):
+    gates = _randn(2, 16)
+    with torch.inference_mode():
+        c = torch.zeros(2, 4, device=cuda_device)
+        h, _ = plstm.gated_scan_step(gates, c, out_c=c)
+    want_h, want_c = plstm.gated_scan_step(gates, torch.zeros(2, 4, device=cuda_device))
+    assert torch.equal(h, want_h) and torch.equal(c, want_c)

@@ -113,3 +113,22 @@ def test_negative_lengths_are_zero(stand_in):
     values = [-1, -(2 ** 31) - 7, torch.iinfo(torch.int64).min]
     ops.gated_scan(torch.zeros(3, 5, 8), lengths=torch.tensor(values))
     assert all(v <= 0 for v in stand_in.lengths[0])
+
+
+# ---- writes into the caller's state --------------------------------------------------------------------
+def test_step_in_place_raises_the_states_version(stand_in):
+    """A graph that saved a state must not differentiate with the step's values."""
+    c = torch.zeros(2, 4, requires_grad=True)
+    state = c + 1
+    loss = (state ** 2).sum()
+    with torch.no_grad():
+        ops.gated_scan_step(torch.zeros(2, 16), state, out_c=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_step_in_place_takes_inference_tensors(stand_in):
+    with torch.inference_mode():
+        c = torch.zeros(2, 4)
+        assert ops.gated_scan_step(torch.zeros(2, 16), c, out_c=c)[1] is c
+    assert ops.gated_scan_step(torch.zeros(2, 16), c, out_c=c)[1] is c

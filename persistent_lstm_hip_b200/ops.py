@@ -175,7 +175,8 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
     gates = _cuda_float(gates, "gates")
     if gates.dim() != 2:
         raise ValueError(f"gates must be [B, 4H], got {tuple(gates.shape)}")
-    if torch.is_grad_enabled() and (gates.requires_grad or c.requires_grad):
+    if torch.is_grad_enabled() and (gates.requires_grad or c.requires_grad or
+                                    (out_c is not None and out_c.requires_grad)):
         if out_c is not None:
             raise ValueError("gated_scan_step with out_c is not differentiable; call it without out_c or under "
                              "no_grad")

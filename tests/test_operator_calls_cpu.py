@@ -132,3 +132,14 @@ def test_step_in_place_takes_inference_tensors(stand_in):
         c = torch.zeros(2, 4)
         assert ops.gated_scan_step(torch.zeros(2, 16), c, out_c=c)[1] is c
     assert ops.gated_scan_step(torch.zeros(2, 16), c, out_c=c)[1] is c
+
+
+@pytest.mark.parametrize("which", ["gates", "c", "out_c"])
+def test_step_in_place_refuses_what_autograd_records(stand_in, which):
+    """Also an out_c of its own that requires a gradient: its graph would belong to other values."""
+    t = dict(gates=torch.zeros(2, 16), c=torch.zeros(2, 4), out_c=torch.zeros(2, 4))
+    t[which].requires_grad_(True)
+    with pytest.raises(ValueError, match="differentiable"):
+        ops.gated_scan_step(t["gates"], t["c"], out_c=t["out_c"])
+    with torch.no_grad():
+        ops.gated_scan_step(t["gates"], t["c"], out_c=t["out_c"])

@@ -17,6 +17,7 @@ import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -31,12 +32,21 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
     lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
+def _refuse_tangents(*tensors) -> None:
+    """The kernels carry no forward-mode tangents, and a result without one would read as a derivative of zero."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("this operator has no forward-mode derivative")
+
+
 def _first_order(backward):
     """once_differentiable, whose bookkeeping only a backward that is itself recorded needs."""
     recorded = once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        _refuse_tangents(*grads)
         return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -161,6 +171,7 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
             raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
         top = gates.shape[0 if seq_major else 1]
         lengths = _fit_lengths(lengths, top).to(device=gates.device, dtype=torch.int32).contiguous()
+    _refuse_tangents(gates, c0)
     if torch.is_grad_enabled() and (gates.requires_grad or (c0 is not None and c0.requires_grad)):
         return _GatedScan.apply(gates, c0, (lengths, plan, seq_major))
     return _scan_forward(plan, gates, c0, lengths, False)[:2]
@@ -175,6 +186,7 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
     gates = _cuda_float(gates, "gates")
     if gates.dim() != 2:
         raise ValueError(f"gates must be [B, 4H], got {tuple(gates.shape)}")
+    _refuse_tangents(gates, c, out_c)
     if torch.is_grad_enabled() and (gates.requires_grad or c.requires_grad or
                                     (out_c is not None and out_c.requires_grad)):
         if out_c is not None:
@@ -277,6 +289,7 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
         residual = _cuda_float(residual, "residual").contiguous()
         _check_residual(residual, x)
     drop = _drop_desc(p, seed, offset, x.device)
+    _refuse_tangents(x, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, (drop, seed if isinstance(seed, torch.Tensor) else None))
     return _dropout(x, drop, residual, x.dtype if residual is None else residual.dtype)
@@ -433,6 +446,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """
     x = _cuda_float(x, "x")
     rows, _, weight, bias, plan = _norm_inputs(x, None, weight, bias, eps)
+    _refuse_tangents(x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, (plan, eps))
@@ -455,6 +469,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
     _check_residual(residual, x)
     x2, r2, weight, bias, plan = _norm_inputs(x, residual, weight, bias, eps)
     drop = _drop_desc(p, seed, offset, x.device)
+    _refuse_tangents(x, residual, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
                                     (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):

@@ -7,6 +7,7 @@ import types
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from persistent_lstm_hip_b200 import _lib, ops
 
@@ -143,3 +144,47 @@ def test_step_in_place_refuses_what_autograd_records(stand_in, which):
         ops.gated_scan_step(t["gates"], t["c"], out_c=t["out_c"])
     with torch.no_grad():
         ops.gated_scan_step(t["gates"], t["c"], out_c=t["out_c"])
+
+
+# ---- forward mode ---------------------------------------------------------------------------------------
+def _one_argument_calls():
+    """(the call as a function of one argument, that argument) for every argument that could carry a derivative."""
+    g, x, c, w = torch.zeros(2, 5, 16), torch.zeros(4, 16), torch.zeros(2, 4), torch.zeros(16)
+    return {
+        "scan gates": (ops.gated_scan, g),
+        "scan c0": (lambda v: ops.gated_scan(g, v), c),
+        "step gates": (lambda v: ops.gated_scan_step(v, c), g[:, 0].clone()),
+        "step c": (lambda v: ops.gated_scan_step(g[:, 0], v), c),
+        "step out_c": (lambda v: ops.gated_scan_step(g[:, 0], c, out_c=v), c),
+        "norm x": (ops.layer_norm, x),
+        "norm weight": (lambda v: ops.layer_norm(x, v), w),
+        "norm bias": (lambda v: ops.layer_norm(x, None, v), w),
+        "dropout x": (lambda v: ops.dropout(v, 0.5, 1), x),
+        "dropout residual": (lambda v: ops.dropout(x, 0.5, 1, residual=v), x),
+        "fused x": (lambda v: ops.dropout_add_layer_norm(v, x), x),
+        "fused residual": (lambda v: ops.dropout_add_layer_norm(x, v), x),
+        "fused weight": (lambda v: ops.dropout_add_layer_norm(x, x, v), w),
+        "fused bias": (lambda v: ops.dropout_add_layer_norm(x, x, None, v), w),
+    }
+
+
+@pytest.mark.parametrize("name", list(_one_argument_calls()))
+def test_forward_mode_is_refused(stand_in, name):
+    """Grad mode says nothing about tangents: no_grad keeps them."""
+    call, v = _one_argument_calls()[name]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(v.clone(), torch.ones_like(v))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+        call(v)  # a level without tangents takes the call
+
+
+def test_tangents_of_a_gradient_are_refused(stand_in):
+    x = torch.zeros(4, 16, requires_grad=True)
+    y = ops.dropout(x, 0.5, 1)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(4, 16), torch.ones(4, 16))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, dual)

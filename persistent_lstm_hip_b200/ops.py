@@ -19,6 +19,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 from .core import _DTYPES, _ptr, _require_cuda
@@ -40,6 +41,13 @@ def _refuse_tangents(*tensors) -> None:
                 raise NotImplementedError("this operator has no forward-mode derivative")
 
 
+def _refuse_tracing() -> None:
+    """A tracer (torch.jit.trace, make_fx) sees the allocations but not the launches: what it records would return
+    uninitialised memory."""
+    if torch._C._is_tracing() or get_proxy_mode() is not None:
+        raise RuntimeError("this operator cannot be traced: its kernel is launched outside of torch's dispatcher")
+
+
 def _first_order(backward):
     """once_differentiable, whose bookkeeping only a backward that is itself recorded needs."""
     recorded = once_differentiable(backward)
@@ -47,6 +55,7 @@ def _first_order(backward):
     @functools.wraps(backward)
     def run(ctx, *grads):
         _refuse_tangents(*grads)
+        _refuse_tracing()
         return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -160,6 +169,7 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
     zero there, and neither the gates nor their gradient count.  Returns h in the gates' type and
     layout and c_n [B,H] f32.  Differentiable in gates and c0.
     """
+    _refuse_tracing()
     gates = _cuda_float(gates, "gates")
     plan = _scan_plan(gates.shape, gates.stride(), gates.dtype, gates.device.index, seq_major)
     if c0 is not None:
@@ -183,6 +193,7 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
 
     out_c (f32 [B,H], contiguous) receives the new state; out_c=c updates the state in place.
     """
+    _refuse_tracing()
     gates = _cuda_float(gates, "gates")
     if gates.dim() != 2:
         raise ValueError(f"gates must be [B, 4H], got {tuple(gates.shape)}")
@@ -284,6 +295,7 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
     when the tensor is advanced before the next replay).  The residual (x's type or f32) sets the
     result's type.  Differentiable in x and residual.
     """
+    _refuse_tracing()
     x = _cuda_float(x, "x").contiguous()
     if residual is not None:
         residual = _cuda_float(residual, "residual").contiguous()
@@ -444,6 +456,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     weight and bias: x's type or f32.  Statistics, and the sums behind the weights' gradients,
     are f32.  Differentiable in x, weight and bias.
     """
+    _refuse_tracing()
     x = _cuda_float(x, "x")
     rows, _, weight, bias, plan = _norm_inputs(x, None, weight, bias, eps)
     _refuse_tangents(x, weight, bias)
@@ -464,6 +477,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
     stored z.  The residual stream may be f32 under a 16-bit x; z has its type, y has x's.
     Differentiable in x, residual, weight and bias.
     """
+    _refuse_tracing()
     x = _cuda_float(x, "x")
     residual = _cuda_float(residual, "residual")
     _check_residual(residual, x)

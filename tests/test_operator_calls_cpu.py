@@ -8,6 +8,7 @@ import types
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from persistent_lstm_hip_b200 import _lib, ops
 
@@ -188,3 +189,26 @@ def test_tangents_of_a_gradient_are_refused(stand_in):
         dual = forward_ad.make_dual(torch.ones(4, 16), torch.ones(4, 16))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, dual)
+
+
+# ---- tracing --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name", list(_one_argument_calls()))
+def test_tracing_is_refused(stand_in, name):
+    """What a tracer records of these calls is their allocations: replaying it gives uninitialised memory, and of a
+    recorded call a plan for one shape."""
+    call, v = _one_argument_calls()[name]
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (v,), check_trace=False)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (v,), check_trace=False)
+    for pre_dispatch in (False, True):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(lambda a: call(a), pre_dispatch=pre_dispatch)(v)
+    call(v)
+
+
+def test_tracing_a_backward_is_refused(stand_in):
+    x = torch.zeros(4, 16, requires_grad=True)
+    y = ops.dropout(x, 0.5, 1)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda dy: torch.autograd.grad(y, x, dy))(torch.ones(4, 16))

@@ -366,11 +366,11 @@ def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, cols: int) -> tor
     return w.contiguous()
 
 
-def _norm_forward(x, residual, weight, bias, plan, drop, keep):
-    """x, residual [rows, cols] -> (y, z or None, stats or None)."""
+def _norm_forward(x, residual, weight, bias, plan, drop, keep, shape):
+    """x, residual [rows, cols] -> (y, z or None, stats or None), y and z of the given shape."""
     dev = x.device
-    y = _empty(plan.rows, dtype=x.dtype, device=dev)
-    z = None if residual is None else _empty(plan.rows, dtype=residual.dtype, device=dev)
+    y = _empty(shape, dtype=x.dtype, device=dev)
+    z = None if residual is None else _empty(shape, dtype=residual.dtype, device=dev)
     stats = _empty(plan.stats, dtype=_F32, device=dev) if keep else None
     rc = _lib.load().plstm_layer_norm_forward(
         plan.desc, None if drop is None else _byref(drop), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
@@ -406,10 +406,11 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, how):
         plan, eps = how
         rows = _rows(x)
-        y, _, stats = _norm_forward(rows, None, weight, bias, plan, None, True)
+        # Not a view of rows: autograd refuses in-place operations on a view that a function returns.
+        y, _, stats = _norm_forward(rows, None, weight, bias, plan, None, True, x.shape)
         ctx.save_for_backward(rows, weight, stats)
         ctx.args = (eps, plan.w_dtype)
-        return y if x.dim() == 2 else y.view(x.shape)
+        return y
 
     @staticmethod
     @_first_order
@@ -426,11 +427,11 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, how):
         plan, drop, seed, eps = how
-        y, z, stats = _norm_forward(_rows(x), _rows(residual), weight, bias, plan, drop, True)
+        y, z, stats = _norm_forward(_rows(x), _rows(residual), weight, bias, plan, drop, True, x.shape)
         ctx.save_for_backward(z, weight, stats, seed)
         ctx.args = (drop, eps, x.dtype, plan.w_dtype)
         ctx.set_materialize_grads(False)
-        return (y, z) if x.dim() == 2 else (y.view(x.shape), z.view(x.shape))
+        return y, z
 
     @staticmethod
     @_first_order
@@ -439,7 +440,8 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
         drop, eps, x_dtype, w_dtype = ctx.args
         if dy is None and dz is None:
             return (None,) * 5
-        shape = (dz if dy is None else dy).shape
+        shape = z.shape
+        z = _rows(z)
         dy = torch.zeros((1, z.shape[1]), dtype=x_dtype, device=z.device).expand(z.shape) if dy is None else _rows(dy)
         dx, dres, dw, db = _norm_backward(z, weight, stats, dy, None if dz is None else _rows(dz), eps,
                                           _saved_drop(drop, seed), x_dtype, w_dtype, ctx.needs_input_grad)
@@ -463,8 +465,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, (plan, eps))
-    y = _norm_forward(rows, None, weight, bias, plan, None, False)[0]
-    return y if x.dim() == 2 else y.view(x.shape)
+    return _norm_forward(rows, None, weight, bias, plan, None, False, x.shape)[0]
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -489,5 +490,4 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
                                     (bias is not None and bias.requires_grad)):
         return _DropoutAddLayerNorm.apply(x, residual, weight, bias,
                                           (plan, drop, seed if isinstance(seed, torch.Tensor) else None, eps))
-    y, z, _ = _norm_forward(x2, r2, weight, bias, plan, drop, False)
-    return (y, z) if x.dim() == 2 else (y.view(x.shape), z.view(x.shape))
+    return _norm_forward(x2, r2, weight, bias, plan, drop, False, x.shape)[:2]

@@ -93,3 +93,16 @@ def test_step_in_inference_mode(cuda_device):
         h, _ = plstm.gated_scan_step(gates, c, out_c=c)
     want_h, want_c = plstm.gated_scan_step(gates, torch.zeros(2, 4, device=cuda_device))
     assert torch.equal(h, want_h) and torch.equal(c, want_c)
+
+
+# ---- in-place operations on results -----------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(16,), (4, 16), (2, 3, 16), (3, 0, 16)])
+def test_in_place_operations_on_results(cuda_device, shape):
+    x, w, res = _randn(*shape).requires_grad_(True), _randn(16, seed=1).requires_grad_(True), _randn(*shape, seed=2)
+    for call in (lambda: plstm.layer_norm(x, w), lambda: plstm.dropout_add_layer_norm(x, res, w, None, 0.25, 3)[0],
+                 lambda: plstm.dropout(x, 0.25, 3) * w):
+        want = call().relu()
+        got = call().relu_()
+        assert got.shape == shape and torch.equal(got, want)
+        grads = [torch.autograd.grad(y, (x, w), torch.ones_like(y)) for y in (got, want)]
+        assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -212,3 +212,38 @@ def test_tracing_a_backward_is_refused(stand_in):
     y = ops.dropout(x, 0.5, 1)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(lambda dy: torch.autograd.grad(y, x, dy))(torch.ones(4, 16))
+
+
+# ---- in-place operations on results -----------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(16,), (4, 16), (2, 3, 16), (2, 2, 3, 16)])
+def test_results_take_in_place_operations(stand_in, shape):
+    """relu_ on a result in training, whatever its axes: no result is a view made inside a function."""
+    x, w = torch.zeros(shape, requires_grad=True), torch.ones(16, requires_grad=True)
+    y = ops.layer_norm(x, w)
+    assert y.shape == shape
+    y.relu_()
+    assert torch.autograd.grad(y.sum(), (x, w))[0].shape == shape
+    y, z = ops.dropout_add_layer_norm(x, torch.zeros(shape), w)
+    assert y.shape == z.shape == shape
+    y.relu_()
+    assert torch.autograd.grad(y.sum() + z.sum(), (x, w))[0].shape == shape
+    y = ops.dropout(x, 0.5, 1)
+    y.relu_()
+    assert torch.autograd.grad(y.sum(), x)[0].shape == shape
+
+
+def test_scan_results_take_in_place_operations(stand_in):
+    gates = torch.zeros(2, 5, 16, requires_grad=True)
+    ops.gated_scan(gates)[0].relu_()
+    h, c = ops.gated_scan_step(gates[:, 0], torch.zeros(2, 4))
+    h.relu_()
+    c.mul_(2)
+
+
+def test_changing_the_saved_residual_stream_is_noticed(stand_in):
+    """The backward needs z as it was."""
+    x = torch.zeros(2, 3, 16, requires_grad=True)
+    y, z = ops.dropout_add_layer_norm(x, torch.zeros(2, 3, 16))
+    z.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

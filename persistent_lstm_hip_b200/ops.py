@@ -177,7 +177,8 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
         if c0.shape != plan.state:
             raise ValueError(f"c0 must be {list(plan.state)}, got {tuple(c0.shape)}")
     if lengths is not None:
-        if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.shape != plan.state[:1]:
+        if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.is_complex() or \
+                lengths.shape != plan.state[:1]:
             raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
         top = gates.shape[0 if seq_major else 1]
         lengths = _fit_lengths(lengths, top).to(device=gates.device, dtype=torch.int32).contiguous()

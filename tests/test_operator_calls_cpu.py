@@ -117,6 +117,12 @@ def test_negative_lengths_are_zero(stand_in):
     assert all(v <= 0 for v in stand_in.lengths[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.complex64])
+def test_lengths_that_are_no_integers_are_refused(stand_in, dtype):
+    with pytest.raises(ValueError, match="lengths"):
+        ops.gated_scan(torch.zeros(2, 5, 8), lengths=torch.ones(2, dtype=dtype))
+
+
 # ---- writes into the caller's state --------------------------------------------------------------------
 def test_step_in_place_raises_the_states_version(stand_in):
     """A graph that saved a state must not differentiate with the step's values."""

@@ -133,12 +133,15 @@ __device__ __forceinline__ F<V> tanh_f(F<V> x) {
   tanh_parts<PRECISE>(x, num, den);
   return num * each(den, rcp);
 }
-// sigmoid(a) tanh(x) with one reciprocal.
+// sigmoid(a) tanh(x) with one reciprocal.  The product of the two denominators, up to 2^128 and 2^26.3, is taken
+// 2^-27 times, so that it passes f32's range only where the result is below 2^-126; undoing that afterwards is
+// exact (and after the product with num, which may be as small as x).
 template <bool PRECISE, int V>
 __device__ __forceinline__ F<V> sigmoid_tanh(F<V> a, F<V> x) {
   F<V> num, den;
   tanh_parts<PRECISE>(x, num, den);
-  return num * each(one_plus(exp_of<PRECISE>(a, -1.0f)) * den, rcp);
+  constexpr float kDown = 1.0f / (1 << 27);
+  return num * each(fma(exp_of<PRECISE>(a, -1.0f), F<V>::of(kDown), kDown) * den, rcp) * F<V>::of(kDown);
 }
 
 template <int V>

@@ -711,7 +711,7 @@ int32_t plstm_layer_norm_forward(const plstm_norm_desc* d, const plstm_dropout_d
                                  const void* residual, const void* weight, const void* bias, void* z, void* y,
                                  float* stats, void* stream) {
   clear_error();
-  const bool fused = residual != nullptr;
+  const bool fused = residual != nullptr || (d != nullptr && d->rows == 0);  // without rows a residual may be NULL
   if (const int32_t rc = check_desc(d, fused)) return rc;
   PLSTM_CHECK_ARG(fused || drop == nullptr, "layer norm: dropout needs a residual");
   NormArgs a{};

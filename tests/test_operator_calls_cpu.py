@@ -253,3 +253,15 @@ def test_changing_the_saved_residual_stream_is_noticed(stand_in):
     z.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+# ---- no rows ------------------------------------------------------------------------------------------------
+def test_fused_step_without_rows_may_have_no_residual_pointer():
+    """An empty tensor's pointer is NULL, and the call still the fused one (returns before any CUDA call)."""
+    lib, drop = _lib.load(), ctypes.byref(_lib.DropoutDesc(0.5, 1, 0, None))
+    for z_dtype in (_lib.F16, _lib.F32):
+        d = ctypes.byref(_lib.NormDesc(0, 8, _lib.F16, z_dtype, _lib.F32, 0, 1e-5, 8, 8, 8, 8))
+        assert lib.plstm_layer_norm_forward(d, drop, None, None, None, None, None, None, None, None) == 0
+    d = ctypes.byref(_lib.NormDesc(1, 8, _lib.F16, _lib.F16, _lib.F32, 0, 1e-5, 8, 8, 8, 8))
+    assert lib.plstm_layer_norm_forward(d, drop, 16, None, None, None, None, 16, None, None) == _lib.EINVAL
+    assert "residual" in _lib.last_error()

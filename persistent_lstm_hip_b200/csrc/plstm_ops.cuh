@@ -86,10 +86,11 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& v) {
   *reinterpret_cast<typename Word<V * sizeof(T)>::type*>(p) = v.word;
 }
 
-// 1 / sqrt(a): the hardware's approximation and one Newton step.
+// 1 / sqrt(a): the hardware's approximation and one Newton step.  a r comes first: half of a subnormal a is
+// rounded, of the smallest to zero.
 __device__ __forceinline__ float rsqrt_rn(float a) {
   const float r = rsqrtf(a);
-  return a > 0.0f && a < INFINITY ? r * fmaf(-0.5f * a * r, r, 1.5f) : r;
+  return a > 0.0f && a < INFINITY ? r * fmaf(-0.5f * (a * r), r, 1.5f) : r;
 }
 
 inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }

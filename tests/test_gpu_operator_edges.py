@@ -47,3 +47,18 @@ def test_closed_gates_in_16_bits(cuda_device, T, H):
     h_up, _ = plstm.gated_scan(gates, torch.full((2, H), -20.0, device=cuda_device))
     s = forms.scan_forward(f64(gates), torch.full((2, H), -20.0, dtype=torch.float64))
     assert ((f64(h_up) - s["h"]).abs() <= 2.0 ** -7 * s["h"].abs() + 2.0 ** -126).all()
+
+
+# ---- norm without eps of rows whose variance is subnormal -----------------------------------------------
+@pytest.mark.parametrize("k", [0, 1, 2, 3])
+def test_norm_of_a_subnormal_variance(cuda_device, k):
+    """Rows whose mean, squares and variance (2^k of f32's smallest step) are exact: what is left is the reciprocal
+    square root and two products, a few units in 2^-24."""
+    n, a = 16 >> k, 2.0 ** -73
+    x = torch.zeros(1, n)
+    x[0, 0], x[0, 1] = a, -a
+    var = 2 * a * a / n
+    assert var == 2.0 ** (k - 149)
+    y = plstm.layer_norm(x.to(cuda_device), eps=0.0)
+    want = x.double() / var ** 0.5
+    assert ((f64(y) - want).abs() <= 16 * 2.0 ** -24 * want.abs()).all()

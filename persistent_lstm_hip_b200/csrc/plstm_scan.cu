@@ -644,6 +644,11 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
   cfg.dynamicSmemBytes = a.stage_at + (backward ? (kHeld<T, V> && K == kSeg ? 2 * K * kMaxThreads * sizeof(F<V>) : 0)
                                        : staged ? cfg.blockDim.x / 32 * Staged<T, V, K>::kBytes
                                                 : 0);
+  // 48 KB need no allowance: runs, ranks' slots (of up to 32 lanes), and what is held or staged.
+  static_assert((2 * kMaxThreads + 2 * kMaxCluster * 32) * sizeof(Run<V>) +
+                    std::max<size_t>(kHeld<T, V> && K == kSeg ? 2 * K * kMaxThreads * sizeof(F<V>) : 0,
+                                     STAGED ? kMaxThreads / 32 * Staged<T, V, K>::kBytes : 0) <=
+                48 * 1024);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -654,8 +659,6 @@ int32_t launch(bool backward, ScanArgs a, cudaStream_t s) {
   const auto go = [&](auto kernel) -> int32_t {
     if (plan.cluster > 8)  // beyond the portable size: has to be allowed for the kernel
       PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (cfg.dynamicSmemBytes > 48 * 1024)
-      PLSTM_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
     PLSTM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan.cluster));
     note_launches(1);
     return PLSTM_OK;

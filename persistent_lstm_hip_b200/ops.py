@@ -28,6 +28,7 @@ _byref = ctypes.byref
 _empty = torch.empty
 _F32 = torch.float32
 _MASK64 = (1 << 64) - 1
+_MAX32 = (1 << 31) - 1
 # The current stream's handle without building a torch.cuda.Stream: small calls are host-bound.
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     lambda index: torch.cuda.current_stream(index).cuda_stream
@@ -91,6 +92,8 @@ class _ScanPlan(NamedTuple):
 def _scan_plan(shape, strides, dtype, index, seq_major, dh_strides=None) -> _ScanPlan:
     if len(shape) != 3 or shape[2] == 0 or shape[2] % 4:
         raise ValueError(f"gates must be [B, T, 4H] with H >= 1, got {tuple(shape)}")
+    if max(shape) > _MAX32:  # the descriptor's fields would wrap
+        raise ValueError(f"gates must have axes below 2^31, got {tuple(shape)}")
     b, t = (1, 0) if seq_major else (0, 1)
     H = shape[2] // 4
     h = (shape[0], shape[1], H)

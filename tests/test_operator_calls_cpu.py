@@ -265,3 +265,13 @@ def test_fused_step_without_rows_may_have_no_residual_pointer():
     d = ctypes.byref(_lib.NormDesc(1, 8, _lib.F16, _lib.F16, _lib.F32, 0, 1e-5, 8, 8, 8, 8))
     assert lib.plstm_layer_norm_forward(d, drop, 16, None, None, None, None, 16, None, None) == _lib.EINVAL
     assert "residual" in _lib.last_error()
+
+
+# ---- sizes ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("seq_major", [False, True])
+@pytest.mark.parametrize("shape", [(2 ** 32 + 1, 1, 8), (1, 2 ** 32 + 1, 8), (2 ** 31, 1, 8), (1, 1, 2 ** 34 + 4)])
+def test_scan_refuses_axes_beyond_its_descriptor(stand_in, shape, seq_major):
+    """They would wrap in its 32-bit fields: 2^32 + 1 rows to one row."""
+    strides = (shape[1] * shape[2], shape[2], 1)
+    with pytest.raises(ValueError, match="below 2.31"):
+        ops._scan_plan(shape, strides, torch.bfloat16, None, seq_major)

@@ -32,21 +32,23 @@ _MAX32 = (1 << 31) - 1
 # The current stream's handle without building a torch.cuda.Stream: small calls are host-bound.
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     lambda index: torch.cuda.current_stream(index).cuda_stream
+# What says that a tracer may be active, each some 0.1 us (get_proxy_mode alone takes 0.4 us): modes on the
+# dispatcher's stack, and on the one above autograd.
+_is_tracing = torch._C._is_tracing
+_modes = torch._C._len_torch_dispatch_stack
+_early_modes = torch._ops.mode_stack_state_for_pre_dispatch().count
 
 
-def _refuse_tangents(*tensors) -> None:
-    """The kernels carry no forward-mode tangents, and a result without one would read as a derivative of zero."""
+def _refuse_transforms(*tensors) -> None:
+    """Refuses what would lose a call without a word.  The kernels carry no forward-mode tangents, and a result
+    without one reads as a derivative of zero.  A tracer (torch.jit.trace, make_fx) sees the allocations but not the
+    launches, and what it records would return uninitialised memory."""
+    if _is_tracing() or ((_modes() or _early_modes()) and get_proxy_mode() is not None):
+        raise RuntimeError("this operator cannot be traced: its kernel is launched outside of torch's dispatcher")
     if forward_ad._current_level >= 0:
         for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError("this operator has no forward-mode derivative")
-
-
-def _refuse_tracing() -> None:
-    """A tracer (torch.jit.trace, make_fx) sees the allocations but not the launches: what it records would return
-    uninitialised memory."""
-    if torch._C._is_tracing() or get_proxy_mode() is not None:
-        raise RuntimeError("this operator cannot be traced: its kernel is launched outside of torch's dispatcher")
 
 
 def _first_order(backward):
@@ -55,8 +57,7 @@ def _first_order(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
-        _refuse_tangents(*grads)
-        _refuse_tracing()
+        _refuse_transforms(*grads)
         return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -172,7 +173,7 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
     zero there, and neither the gates nor their gradient count.  Returns h in the gates' type and
     layout and c_n [B,H] f32.  Differentiable in gates and c0.
     """
-    _refuse_tracing()
+    _refuse_transforms(gates, c0)
     gates = _cuda_float(gates, "gates")
     plan = _scan_plan(gates.shape, gates.stride(), gates.dtype, gates.device.index, seq_major)
     if c0 is not None:
@@ -185,7 +186,6 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
             raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
         top = gates.shape[0 if seq_major else 1]
         lengths = _fit_lengths(lengths, top).to(device=gates.device, dtype=torch.int32).contiguous()
-    _refuse_tangents(gates, c0)
     if torch.is_grad_enabled() and (gates.requires_grad or (c0 is not None and c0.requires_grad)):
         return _GatedScan.apply(gates, c0, (lengths, plan, seq_major))
     return _scan_forward(plan, gates, c0, lengths, False)[:2]
@@ -197,11 +197,10 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
 
     out_c (f32 [B,H], contiguous) receives the new state; out_c=c updates the state in place.
     """
-    _refuse_tracing()
+    _refuse_transforms(gates, c, out_c)
     gates = _cuda_float(gates, "gates")
     if gates.dim() != 2:
         raise ValueError(f"gates must be [B, 4H], got {tuple(gates.shape)}")
-    _refuse_tangents(gates, c, out_c)
     if torch.is_grad_enabled() and (gates.requires_grad or c.requires_grad or
                                     (out_c is not None and out_c.requires_grad)):
         if out_c is not None:
@@ -299,13 +298,12 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
     when the tensor is advanced before the next replay).  The residual (x's type or f32) sets the
     result's type.  Differentiable in x and residual.
     """
-    _refuse_tracing()
+    _refuse_transforms(x, residual)
     x = _cuda_float(x, "x").contiguous()
     if residual is not None:
         residual = _cuda_float(residual, "residual").contiguous()
         _check_residual(residual, x)
     drop = _drop_desc(p, seed, offset, x.device)
-    _refuse_tangents(x, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, (drop, seed if isinstance(seed, torch.Tensor) else None))
     return _dropout(x, drop, residual, x.dtype if residual is None else residual.dtype)
@@ -370,6 +368,11 @@ def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, cols: int) -> tor
     return w.contiguous()
 
 
+def _shape(x, plan) -> tuple:
+    """x's shape (as a tuple: torch.empty takes 1 us more for a torch.Size)."""
+    return plan.rows if x.dim() == 2 else tuple(x.shape)
+
+
 def _norm_forward(x, residual, weight, bias, plan, drop, keep, shape):
     """x, residual [rows, cols] -> (y, z or None, stats or None), y and z of the given shape."""
     dev = x.device
@@ -411,7 +414,7 @@ class _LayerNorm(torch.autograd.Function):
         plan, eps = how
         rows = _rows(x)
         # Not a view of rows: autograd refuses in-place operations on a view that a function returns.
-        y, _, stats = _norm_forward(rows, None, weight, bias, plan, None, True, x.shape)
+        y, _, stats = _norm_forward(rows, None, weight, bias, plan, None, True, _shape(x, plan))
         ctx.save_for_backward(rows, weight, stats)
         ctx.args = (eps, plan.w_dtype)
         return y
@@ -431,7 +434,8 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, how):
         plan, drop, seed, eps = how
-        y, z, stats = _norm_forward(_rows(x), _rows(residual), weight, bias, plan, drop, True, x.shape)
+        y, z, stats = _norm_forward(_rows(x), _rows(residual), weight, bias, plan, drop, True,
+                                    _shape(x, plan))
         ctx.save_for_backward(z, weight, stats, seed)
         ctx.args = (drop, eps, x.dtype, plan.w_dtype)
         ctx.set_materialize_grads(False)
@@ -462,14 +466,13 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     weight and bias: x's type or f32.  Statistics, and the sums behind the weights' gradients,
     are f32.  Differentiable in x, weight and bias.
     """
-    _refuse_tracing()
+    _refuse_transforms(x, weight, bias)
     x = _cuda_float(x, "x")
     rows, _, weight, bias, plan = _norm_inputs(x, None, weight, bias, eps)
-    _refuse_tangents(x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, (plan, eps))
-    return _norm_forward(rows, None, weight, bias, plan, None, False, x.shape)[0]
+    return _norm_forward(rows, None, weight, bias, plan, None, False, _shape(x, plan))[0]
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -482,16 +485,15 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
     stored z.  The residual stream may be f32 under a 16-bit x; z has its type, y has x's.
     Differentiable in x, residual, weight and bias.
     """
-    _refuse_tracing()
+    _refuse_transforms(x, residual, weight, bias)
     x = _cuda_float(x, "x")
     residual = _cuda_float(residual, "residual")
     _check_residual(residual, x)
     x2, r2, weight, bias, plan = _norm_inputs(x, residual, weight, bias, eps)
     drop = _drop_desc(p, seed, offset, x.device)
-    _refuse_tangents(x, residual, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
                                     (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _DropoutAddLayerNorm.apply(x, residual, weight, bias,
                                           (plan, drop, seed if isinstance(seed, torch.Tensor) else None, eps))
-    return _norm_forward(x2, r2, weight, bias, plan, drop, False, x.shape)[:2]
+    return _norm_forward(x2, r2, weight, bias, plan, drop, False, _shape(x, plan))[:2]

@@ -107,6 +107,12 @@ def _scan_plan(shape, strides, dtype, index, seq_major, dh_strides=None) -> _Sca
     return _ScanPlan(_byref(d), (shape[b], H), h, nbytes.value // 4, d)
 
 
+@_plan
+def _step_plan(shape, strides, dtype, index) -> _ScanPlan:
+    """One step of [1, B, 4H]; h is allocated without the axis of one."""
+    return _scan_plan((1, *shape), (0, *strides), dtype, index, True)
+
+
 def _scan_forward(plan, gates, c0, lengths, keep):
     dev = gates.device
     h = _empty(plan.h, dtype=gates.dtype, device=dev)
@@ -208,9 +214,8 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
                              "no_grad")
         h, c_n = gated_scan(gates[:, None], c)
         return h[:, 0], c_n
-    # One step of [1, B, 4H]; h is allocated without the axis of one.
     dev = gates.device
-    plan = _scan_plan((1, *gates.shape), (0, *gates.stride()), gates.dtype, dev.index, True)
+    plan = _step_plan(gates.shape, gates.stride(), gates.dtype, dev.index)
     c = _require_cuda(c, "c", dev, _F32)
     if c.shape != plan.state:
         raise ValueError(f"c must be {list(plan.state)}, got {tuple(c.shape)}")
@@ -342,29 +347,28 @@ def _norm_inputs(x, residual, weight, bias, eps):
     """Checks the arguments; x and residual as rows, contiguous weights, and their plan."""
     if x.dim() == 0:
         raise ValueError("x must have at least one axis")
-    cols = x.shape[-1]
+    cols, dev, dtype = x.shape[-1], x.device, x.dtype
     w_dtype = None
     if weight is not None:
         w_dtype = weight.dtype
-        weight = _check_weight(weight, "weight", x, cols)
+        weight = _check_weight(weight, "weight", dev, dtype, cols)
     if bias is not None:
         if w_dtype is not None and bias.dtype is not w_dtype:
             raise ValueError("weight and bias must have one dtype")
         w_dtype = bias.dtype
-        bias = _check_weight(bias, "bias", x, cols)
+        bias = _check_weight(bias, "bias", dev, dtype, cols)
     x2 = _rows(x) if cols else x.reshape(0, 0)
     r2 = None if residual is None else _rows(residual)
-    dtype = x.dtype
-    plan = _norm_plan(x2.shape[0], cols, dtype, dtype if r2 is None else r2.dtype, w_dtype or dtype, x.device.index,
-                      eps, x2.stride(0), 0 if r2 is None else r2.stride(0))
+    plan = _norm_plan(x2.shape[0], cols, dtype, dtype if r2 is None else r2.dtype, w_dtype or dtype, dev.index, eps,
+                      x2.stride(0), 0 if r2 is None else r2.stride(0))
     return x2, r2, weight, bias, plan
 
 
-def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, cols: int) -> torch.Tensor:
-    if w.dim() != 1 or w.shape[0] != cols or w.device != x.device:
-        raise ValueError(f"{name} must be [{cols}] on {x.device}, got {tuple(w.shape)} on {w.device}")
-    if w.dtype is not x.dtype and w.dtype is not _F32:
-        raise ValueError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
+def _check_weight(w: torch.Tensor, name: str, dev: torch.device, dtype: torch.dtype, cols: int) -> torch.Tensor:
+    if w.dim() != 1 or w.shape[0] != cols or w.device != dev:
+        raise ValueError(f"{name} must be [{cols}] on {dev}, got {tuple(w.shape)} on {w.device}")
+    if w.dtype is not dtype and w.dtype is not _F32:
+        raise ValueError(f"{name} must be {dtype} or float32, got {w.dtype}")
     return w.contiguous()
 
 

@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
-from .core import _DTYPES, _ptr, _require_cuda
+from .core import _DTYPES, _require_cuda
 
 _byref = ctypes.byref
 _empty = torch.empty
@@ -67,6 +67,18 @@ def _first_order(backward):
 # What depends on shapes, strides and types alone (checks, descriptors, sizes) is worked out once for
 # each combination and found again by it in these bounded caches.
 _plan = functools.lru_cache(maxsize=512)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    """The address of a tensor's elements, NULL for None.  Tensors without memory of their own (DTensor and other
+    wrappers) have no address, and NULL would read as an argument left out (where none may be, the library refuses
+    it)."""
+    if t is None:
+        return None
+    address = t.data_ptr()
+    if not address and t.numel():
+        raise ValueError(f"a {type(t).__name__} without memory of its own is not supported; pass a plain tensor")
+    return address
 
 
 def _cuda_float(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -228,7 +240,7 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
         # The kernel writes behind autograd's back: a graph that saved this state has to notice.
         torch.autograd.graph.increment_version(out_c)
     h = _empty(plan.state, dtype=gates.dtype, device=dev)
-    rc = _lib.load().plstm_gated_scan_forward(plan.desc, gates.data_ptr(), None, c.data_ptr(), h.data_ptr(),
+    rc = _lib.load().plstm_gated_scan_forward(plan.desc, gates.data_ptr(), None, _ptr(c), h.data_ptr(),
                                               out_c.data_ptr(), None, _stream(dev.index))
     if rc:
         _lib.check(rc)
@@ -244,7 +256,7 @@ def _drop_desc(p: float, seed: Union[int, torch.Tensor], offset: int, device: to
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise ValueError(f"a tensor seed must be one int64 on {device}")
-        return _lib.DropoutDesc(p, 0, offset, seed.data_ptr())
+        return _lib.DropoutDesc(p, 0, offset, _ptr(seed))
     if not 0 <= seed <= _MASK64:
         raise ValueError("seed must be in [0, 2^64)")
     return _lib.DropoutDesc(p, seed, offset, None)
@@ -253,7 +265,7 @@ def _drop_desc(p: float, seed: Union[int, torch.Tensor], offset: int, device: to
 def _saved_drop(drop, seed):
     """The forward's descriptor for its backward.  A tensor seed is read where autograd holds it: saved-tensor
     hooks (checkpointing, offloading) keep a copy, and the forward's own tensor may be changed or freed by then."""
-    return drop if seed is None else _lib.DropoutDesc(drop.p, 0, drop.offset, seed.data_ptr())
+    return drop if seed is None else _lib.DropoutDesc(drop.p, 0, drop.offset, _ptr(seed))
 
 
 def _dropout(x, drop, residual, dtype):

@@ -275,3 +275,42 @@ def test_scan_refuses_axes_beyond_its_descriptor(stand_in, shape, seq_major):
     strides = (shape[1] * shape[2], shape[2], 1)
     with pytest.raises(ValueError, match="below 2.31"):
         ops._scan_plan(shape, strides, torch.bfloat16, None, seq_major)
+
+
+# ---- tensors without memory of their own --------------------------------------------------------------------
+class Wrapper(torch.Tensor):
+    """As DTensor and others are built: operations reach the inner tensor, data_ptr() is 0."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        args = [a.inner if isinstance(a, Wrapper) else a for a in args]
+        return Wrapper(func(*args, **(kwargs or {})))
+
+
+# The rest (gates, x, out_c) may not be left out, and the library refuses a NULL there.
+_OPTIONAL = ("scan c0", "step c", "norm weight", "norm bias", "dropout residual", "fused residual", "fused weight",
+             "fused bias")
+_WRAPPED_CALLS = {
+    **{name: _one_argument_calls()[name] for name in _OPTIONAL},
+    "scan lengths": (lambda v: ops.gated_scan(torch.zeros(2, 5, 16), lengths=v), torch.tensor([1, 2], dtype=torch.int32)),
+    "dropout seed": (lambda v: ops.dropout(torch.zeros(8), 0.5, v), torch.tensor([5])),
+    "fused seed": (lambda v: ops.dropout_add_layer_norm(torch.zeros(2, 8), torch.zeros(2, 8), p=0.5, seed=v),
+                   torch.tensor([5])),
+}
+
+
+@pytest.mark.parametrize("name", list(_WRAPPED_CALLS))
+def test_tensors_without_memory_are_refused(stand_in, name):
+    """Their NULL would read as no weight, no state, no residual, no lengths or the seed 0."""
+    call, v = _WRAPPED_CALLS[name]
+    wrapped = Wrapper(v.clone())
+    assert wrapped.data_ptr() == 0
+    with pytest.raises(ValueError, match="memory of its own"):
+        call(wrapped)

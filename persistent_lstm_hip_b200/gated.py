@@ -59,7 +59,7 @@ class GatedScanRegressor(nn.Module):
 
     def init_state(self, batch: int) -> List[torch.Tensor]:
         dev = self.linear.weight.device
-        return [torch.zeros(batch, self.hidden_dim, device=dev) for _ in self.layers]
+        return [torch.zeros(batch, self.hidden_dim, device=dev, dtype=torch.float32) for _ in self.layers]
 
     def _blocks(self, z, scan, p, seed):
         y = ops.layer_norm(z, self.norm_weight[0], self.norm_bias[0], self.eps)

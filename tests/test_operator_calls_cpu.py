@@ -10,7 +10,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from persistent_lstm_hip_b200 import _lib, ops
+from persistent_lstm_hip_b200 import GatedScanRegressor, _lib, ops
 
 
 class StandIn:
@@ -314,3 +314,15 @@ def test_tensors_without_memory_are_refused(stand_in, name):
     assert wrapped.data_ptr() == 0
     with pytest.raises(ValueError, match="memory of its own"):
         call(wrapped)
+
+
+# ---- states of the regressor ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("default", [torch.float32, torch.float64, torch.bfloat16])
+def test_states_are_f32_whatever_the_default_type(default):
+    m, before = GatedScanRegressor(3, 8, 2, 2), torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        state = m.init_state(4)
+    finally:
+        torch.set_default_dtype(before)
+    assert [(c.dtype, tuple(c.shape)) for c in state] == [(torch.float32, (4, 8))] * 2

@@ -350,7 +350,7 @@ typedef struct plstm_norm_desc {
 } plstm_norm_desc;
 #define PLSTM_NORM_MAX_COLS 16384
 /* weight and bias may be NULL (1 and 0).  residual NULL: plain layer norm, z is not
- * written and drop must be NULL.  drop NULL: no dropout.  stats (f32 [2][rows]: mean,
+ * written and drop must be NULL (but with rows 0 any pointer may be NULL).  drop NULL: no dropout.  stats (f32 [2][rows]: mean,
  * then 1 / sqrt(var + eps)) is what the backward needs, or NULL. */
 PLSTM_API int32_t plstm_layer_norm_forward(const plstm_norm_desc* d, const plstm_dropout_desc* drop, const void* x,
                                            const void* residual, const void* weight, const void* bias, void* z,

@@ -17,7 +17,9 @@ constexpr int kThreads = 256;
 // A thread takes kUnroll groups of eight elements a turn, a CTA's apart, and issues all their loads
 // before it draws: with one 16-byte load in flight a thread the kernel waited on memory (68 to 69 us
 // for 65.5 M f16 elements against 64 us; two groups take 65 to 69 us).  64 us is 63 % of the measured
-// bandwidth: 20 widening products a Philox call keep the multiplier 62 % busy, issue is 57 %.
+// bandwidth: 20 widening products a Philox call keep the multiplier 62 % busy, issue is 57 %.  In f32 as many take
+// 110 us, 73 %, and with a residual 154 us, 78 % (its four groups do not fit 64 registers: 168 bytes spill); f16 with
+// a residual 73 us, 82 %.
 constexpr int kUnroll = 4;
 
 template <typename T>

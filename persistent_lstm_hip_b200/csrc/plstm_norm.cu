@@ -8,12 +8,14 @@
 // The weight gradients are summed per thread over the rows its CTA visits, then over the
 // CTA's row groups, then over the CTAs by a second kernel: a fixed order, no atomics.
 //
-// Both directions are bound by instruction issue before memory.  Measured at 65536 x 1024 bf16 with f32
-// weights: forward 53 us, 78 % of the measured 6.54 TB/s (14 instructions an element); backward with the
-// weight gradients 86 us, 71 % (27 an element).  With residual and dropout at 131072 x 512: 127 and 158 us, 65 %
-// and 65 % (Philox adds 11.5 an element); with f32 throughout at 65536 x 512: 88 and 113 us, 93 % and 91 %.
-// Rows 1001 wide (33000 of them): 57 and 91 us against 26 and 42 us that their bytes would take at the 1024's rate:
-// the masked ends and the columns' places cost instructions.
+// Measured at 65536 x 1024 bf16 with f32 weights: forward 53 us, 78 % of the measured 6.54 TB/s (14 instructions an
+// element, issue 54 %); backward with the weight gradients 86 us, 71 % (27 an element, issue 63 %, 23 % of the warps).
+// With residual and dropout at 131072 x 512: 128 and 157 us, 64 % and 65 % (Philox adds 11.5 instructions an element);
+// the same elements 1024 wide: 165 and 166 us, 50 % and 62 %, where the forward's four chunks a thread spill (make_split)
+// and it waits for memory (issue 46 %); with f32 throughout at 65536 x 512: 88 and 114 us, 94 % and 90 %.
+// Rows 1001 wide (33000 of them, bf16) take 57 and 91 us, rows 1024 wide 31 and 50 us: the masked ends, the columns'
+// places and single reads of the weights cost instructions.  Rows of 16384 (8192 of them, bf16, f32 weights): 156 and
+// 366 us, 53 % and 34 %.
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
@@ -36,7 +38,9 @@ struct Split {
   int ch, tpr, teams;
   int block() const { return tpr * teams; }
 };
-// Widest team: four chunks a thread hold 16384 columns (2049 chunks), two a thread 4096 (513).
+// Widest team: four chunks a thread hold 16384 columns (2049 chunks), two a thread 4096 (513).  The CTA of 544 threads
+// leaves 96 registers to every four-chunk kernel, of whatever width: the plain forwards spill up to 68 bytes, the fused
+// ones 24 to 556, the backwards 48 to 864.
 constexpr int max_block(int ch) { return ch == 4 ? 544 : 288; }
 constexpr int kTeamBlock = 128;  // CTA size up to which teams share a CTA
 
@@ -528,8 +532,8 @@ __global__ void __maxnreg__(backward_registers(CH, sizeof(TV))) norm_backward_ke
 }
 
 // dweight / dbias from the CTAs' partial sums [parts][2][cols]: 32 columns per CTA, 32 threads
-// deep over the parts, then a fixed tree.  Launched while the backward still runs
-// (programmatic dependent launch); it waits for it before it reads.
+// deep over the parts, then a fixed tree.  A programmatic dependent launch: its launch latency lies under the
+// backward, whose last CTA's end is what lets it start (the backward gives no earlier signal).
 __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __restrict__ partial, int parts, int cols,
                                                                 void* dweight, void* dbias, int w_dtype) {
   __shared__ float sums[32][33];
@@ -555,8 +559,8 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __r
 // 60 us with two; the backward 87 us with two (their sums of weight gradients are registers) and
 // 103 us with one.  A few rows are over before that matters, and one chunk is the shortest way
 // (backward of 16 x 512: 6.7 us with one, 9.0 us with two).  The fused forward would rather have two
-// (33000 x 1001: 122 us against 146 us), but it sums in the plain one's order, so that both give the
-// same bits.
+// (33000 x 1001: 122 us against 146 us), but it sums in the plain one's order: where types and alignment
+// are the same, y has the bits of the separate norm of z.
 Split make_split(const plstm_norm_desc& d, bool whole, bool backward) {
   Split s;
   const int chunks = whole ? d.cols / 8 : chunk_columns(d.cols);

@@ -15,16 +15,18 @@
 // steps again out of registers to write h.  The input is read once and the waits are the
 // hardware's barriers.
 //
-// Measured (GPU time, of the measured 6.54 TB/s): forward 169 us for B = 512, T = 1000, H = 128, f16, 59 % (the
-// special-function unit is 68 % busy with its eight instructions an element, the issue slots 59 %); 181 us for
-// one row of 65,536 steps of H = 512, bf16, 28 % (32 turns of a cluster exchange each); 228 us for 1024 rows of
-// 200 to 1000 steps, 59 %.
+// Measured (GPU time, of the measured 6.54 TB/s): forward 168 us for B = 512, T = 1000, H = 128, f16, 60 % (the
+// special-function unit is 69 % busy with its eight instructions an element, the issue slots 59 %; 1024 CTAs are 1.73
+// waves of the 592 that fit), in f32 250 us, 80 %; 183 us for one row of 65,536 steps of H = 512, bf16, 28 % (32 turns,
+// each with a cluster barrier under which only the next turn's copies run); 231 us for 1024 rows of 200 to 1000 steps,
+// 60 %; 31 us for 4096 rows of three steps of H = 512, bf16, 31 %.
 //
 // Backward, with e_t = dh_t o_t (1 - tanh(c_t)^2): dc_t = e_t + G_t, G_{t-1} = f_t dc_t, where
 // G enters the last step as dc_n and leaves the first as dc0: the same composition in reversed
-// time.  c is rebuilt from the state that the forward kept for every segment.  298 us for the first shape
+// time.  c is rebuilt from the state that the forward kept for every segment.  294 us for the first shape
 // above, 61 %: ten special-function instructions an element and 16 warps on an SM, since a step leaves
-// five values for the second pass.
+// five values for the second pass; in f32 481 us, 75 %.  The long row takes 290 us, 32 %, the short ones 47 us, 37 %
+// (64 registers, of which up to 132 bytes spill).
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <initializer_list>
@@ -149,7 +151,7 @@ struct alignas(8 * V) Run {  // the action c -> a c + b of a run of steps
   F<V> a, b;
 };
 
-// Reads V elements; those past the length are given as the step that changes nothing.
+// The type's infinity, for 16 bits twice: with the other gates zero it is the forget gate of a step that changes nothing.
 template <typename T>
 __device__ __forceinline__ uint32_t infinity_bits() {
   return sizeof(T) == 4 ? 0x7f800000u : std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
@@ -309,7 +311,7 @@ __device__ __forceinline__ void load_steps(const T* from, int64_t stride, int H,
 // word [step][gate][lane] is what `lane` will read.  A warp reads only what it copied, so no barrier is
 // needed, and the copies for a turn fly while the turn before is worked on without holding registers.
 // Steps past the length and channels past H arrive as zeros.  The forward stages in clusters, where a turn
-// is long and the warps are few (one row of 65,536 steps, H = 512, bf16: 178 us against 224 us with the next
+// is long and the warps are few (one row of 65,536 steps, H = 512, bf16: a fifth less time than with the next
 // turn in registers); elsewhere the detour costs more than it hides (B = 512, T = 1000, H = 128, f16: 185 us
 // against 168 us), and so it does in the backward.
 template <typename T, int V, int K>
@@ -534,8 +536,8 @@ __global__ void __launch_bounds__(kMaxThreads, K < kSeg ? 8 : CTAS) scan_backwar
 }
 
 // One step of a batch of streams: a thread takes V channels of one row, nothing is exchanged.  16 rows of
-// H = 512 bf16 take 1.8 us, a launch; 4096 rows of H = 2048 24 us, 53 % of the measured bandwidth (the general
-// kernel took 53 us, most of it finding its place).
+// H = 512 bf16 take 1.9 us, a launch; 4096 rows of H = 2048 24 us, 96 % of the measured bandwidth with the f32 state
+// read and written (the general kernel took 53 us, most of it finding its place).
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) scan_step_kernel(const __grid_constant__ ScanArgs p) {
   constexpr bool PRECISE = sizeof(T) == 4;

@@ -6,7 +6,8 @@
 * ``dropout``: from a counter-based generator, so the mask is never stored.
 * ``dropout_add_layer_norm``: the residual step z = residual + dropout(x), y = layer_norm(z).
 
-Inputs are CUDA tensors in f32, f16 or bf16; there is no CPU path.  Work is enqueued on the
+Inputs are CUDA tensors in f32, f16 or bf16; there is no CPU path.  Gradients are of the first
+order and in reverse mode; forward mode, second derivatives and tracers are refused.  Work is enqueued on the
 current stream of the inputs' device.  The scan and the norms read strided batches, time
 steps and rows in place; only a last axis that is not contiguous is copied first.
 """
@@ -213,7 +214,8 @@ def gated_scan_step(gates: torch.Tensor, c: torch.Tensor, *,
                     out_c: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """One time step of ``gated_scan`` for a batch of streams: gates [B,4H], state c [B,H] f32 -> (h, c_new).
 
-    out_c (f32 [B,H], contiguous) receives the new state; out_c=c updates the state in place.
+    out_c (f32 [B,H], contiguous) receives the new state; out_c=c updates the state in place, any other
+    must not overlap c.  Differentiable without out_c.
     """
     _refuse_transforms(gates, c, out_c)
     gates = _cuda_float(gates, "gates")
@@ -497,8 +499,10 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
                            eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
     """The residual step in one pass: z = residual + dropout(x), y = layer_norm(z) -> (y, z).
 
-    Bit for bit dropout(x, p, seed, offset, residual=residual) followed by the norm of that
-    stored z.  The residual stream may be f32 under a 16-bit x; z has its type, y has x's.
+    z is dropout(x, p, seed, offset, residual=residual) bit for bit, and y the norm of that stored
+    z: with a residual of x's type, and rows that start on 16 bytes or are no multiple of eight
+    wide, layer_norm(z, weight, bias, eps) bit for bit; else its sums may run in another order.
+    The residual stream may be f32 under a 16-bit x; z has its type, y has x's.
     Differentiable in x, residual, weight and bias.
     """
     _refuse_transforms(x, residual, weight, bias)

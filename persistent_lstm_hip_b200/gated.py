@@ -78,6 +78,8 @@ class GatedScanRegressor(nn.Module):
         p = self.dropout if self.training else 0.0
         if seed is None:
             seed = int(torch.randint(1 << 62, ())) if p > 0 else 0
+        if lengths is not None:  # once for all layers
+            lengths = ops.lengths32(lengths, x.shape[0], x.shape[1], x.device)
         state_n = []
 
         def scan(l, layer, y):

@@ -170,8 +170,12 @@ class _GatedScan(torch.autograd.Function):
         return dgates, dc0, None
 
 
-def _fit_lengths(lengths: torch.Tensor, top: int) -> torch.Tensor:
-    """`lengths` within int32.  The kernel clamps to [0, top]; what int32 cannot hold is clamped before it would wrap."""
+def lengths32(lengths: torch.Tensor, batch: int, top: int, device: torch.device) -> torch.Tensor:
+    """Checked lengths as the kernels take them: int32 on the device.  The kernels clamp to [0, top]; what int32
+    cannot hold is clamped before it would wrap."""
+    if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.is_complex() or \
+            lengths.shape != (batch,):
+        raise ValueError(f"lengths must be an integer tensor [{batch}]")
     if lengths.dtype is torch.uint64:  # the upper half is negative as int64
         lengths = lengths.to(torch.int64)
         lengths = torch.where(lengths < 0, top, lengths)
@@ -179,7 +183,7 @@ def _fit_lengths(lengths: torch.Tensor, top: int) -> torch.Tensor:
         lengths = lengths.to(torch.int64)
     if lengths.dtype is torch.int64:
         lengths = lengths.clamp(0, top)
-    return lengths
+    return lengths.to(device=device, dtype=torch.int32).contiguous()
 
 
 def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, *,
@@ -200,11 +204,7 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, lengths: 
         if c0.shape != plan.state:
             raise ValueError(f"c0 must be {list(plan.state)}, got {tuple(c0.shape)}")
     if lengths is not None:
-        if not isinstance(lengths, torch.Tensor) or lengths.is_floating_point() or lengths.is_complex() or \
-                lengths.shape != plan.state[:1]:
-            raise ValueError(f"lengths must be an integer tensor [{plan.state[0]}]")
-        top = gates.shape[0 if seq_major else 1]
-        lengths = _fit_lengths(lengths, top).to(device=gates.device, dtype=torch.int32).contiguous()
+        lengths = lengths32(lengths, plan.state[0], gates.shape[0 if seq_major else 1], gates.device)
     if torch.is_grad_enabled() and (gates.requires_grad or (c0 is not None and c0.requires_grad)):
         return _GatedScan.apply(gates, c0, (lengths, plan, seq_major))
     return _scan_forward(plan, gates, c0, lengths, False)[:2]
